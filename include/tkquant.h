@@ -42,12 +42,18 @@ extern "C" {
 #define TKQ_FMT_E2M1 1 /* 2 elements per byte, even index in the low nibble */
 #define TKQ_FMT_E5M6 2 /* 8 elements in 3 little-endian uint32 words */
 
+/* element types of block scales read by the matrix products */
+#define TKQ_SFMT_UE8M0 0 /* exponent bytes (powers of two) */
+#define TKQ_SFMT_E4M3 1  /* float8_e4m3fn */
+
 /* flag bits */
 #define TKQ_ROUND_SF 1u     /* round the scale up to a power of two */
 #define TKQ_SF_COL_MAJOR 2u /* column-major scale storage */
 #define TKQ_SF_UE8M0 4u     /* exponent bytes, four per 32-bit word; needs TKQ_SF_COL_MAJOR */
 #define TKQ_SF_ONLY 8u      /* compute and store scales only; `out` is not touched */
 #define TKQ_CAST_ONLY 16u   /* read row-major fp32 scales from `sf`, store data only */
+#define TKQ_ZERO_GAPS 64u   /* grouped products: rows of no group are set to zero */
+#define TKQ_ACCUMULATE 128u /* weight gradient: add to what `out` holds */
 #define TKQ_EXACT_CODES 32u /* fused SwiGLU cast only: evaluate every activation with the exact routine (see there) */
 
 /* negative return codes */
@@ -324,6 +330,71 @@ int tkq_expand_to_fused(const void* x, int64_t num_tokens, int64_t row_bytes, co
                         const int32_t* token_topk_to_pos, int64_t num_topk, const int32_t* pos_to_expert,
                         int64_t num_expanded_tokens, unsigned flags, void* out, void* out_sf, int64_t out_sf_stride,
                         void* stream);
+
+/*
+ * NVFP4 cast: e2m1 codes with an e4m3 scale per 16 values of a row and one fp32 scale per tensor.  With amax the largest
+ * magnitude of a block: s = nearest e4m3 of amax / (6 ts), at most 448; code = nearest e2m1 of x / (s ts), 0 where s is 0;
+ * both of the exact quotients, ties to even.  No counterpart in the reference (its FP4 scales are powers of two).
+ *
+ *   x             [num_tokens, x_row_stride] bf16 or fp32, rows on 16-byte boundaries; hidden a multiple of 16
+ *   tensor_scale  ts, one fp32 on the device, positive
+ *   out           [num_tokens, hidden / 2] bytes, even index in the low nibble;  sf  [num_tokens, hidden / 16] e4m3 bytes
+ */
+int tkq_per_token_cast_nvfp4(const void* x, int x_dtype, int64_t num_tokens, int64_t hidden, int64_t x_row_stride,
+                             const float* tensor_scale, void* out, void* sf, void* stream);
+
+/* The way back: code * s * ts, rounded once to fp32 and, for bf16, once more.  Layouts as above, out [num_tokens, hidden]. */
+int tkq_cast_back_nvfp4(const void* x, const void* sf, const float* tensor_scale, int64_t num_tokens, int64_t hidden,
+                        int out_dtype, void* out, void* stream);
+
+/*
+ * Products of quantized matrices: out[r, i] = alpha_e * sum_k x[r, k] * w[e, i, k] in fp32, rounded once to bf16, for the
+ * rows r of group e, expert_start[e] <= r < expert_end[e].  The operands stay in their 8- or 4-bit form on the way to the
+ * tensor core, which applies the block scales.  No counterpart in the reference.
+ *
+ *   x                [num_rows, k] and  w [num_experts, n, k]: e4m3 bytes, or e2m1 pairs (strides count values)
+ *   x_sf, w_sf       four scale bytes per 32-bit word along k: word q of row block m at m * row_stride + q * k_stride
+ *                    (+ e * expert_stride for w), strides in words.  The packed column-major storage of the casts has
+ *                    row_stride 1 and k_stride = its pitch in words
+ *   *_block_m        rows per scale: 1, 32 or 128;  *_block_k values per scale: 32 or 128 (e4m3), 32 (e2m1, ue8m0),
+ *                    16 (e2m1, e4m3 scales)
+ *   fmt, sf_fmt      TKQ_FMT_E4M3 or TKQ_FMT_E2M1; TKQ_SFMT_UE8M0, or TKQ_SFMT_E4M3 with e2m1
+ *   expert_start/end int32[num_experts], ascending and disjoint; values outside [0, num_rows] are clamped.  Both NULL with
+ *                    num_experts = 1: one group of all rows
+ *   k                multiple of 32 (e4m3) or 64 (e2m1); data rows start on 16-byte boundaries
+ *   alpha            NULL or fp32, alpha[e * alpha_stride]
+ *   out              bf16 [num_rows, out_row_stride]; rows of no group are left alone, or cleared with TKQ_ZERO_GAPS
+ */
+int tkq_block_scaled_gemm(const void* x, int64_t x_row_stride, const void* x_sf, int64_t x_sf_row_stride, int64_t x_sf_k_stride,
+                          int x_block_m, int x_block_k, const void* w, int64_t w_expert_stride, int64_t w_row_stride,
+                          const void* w_sf, int64_t w_sf_expert_stride, int64_t w_sf_row_stride, int64_t w_sf_k_stride,
+                          int w_block_m, int w_block_k, int fmt, int sf_fmt, const int32_t* expert_start,
+                          const int32_t* expert_end, int64_t num_experts, int64_t num_rows, int64_t n, int64_t k,
+                          const float* alpha, int64_t alpha_stride, void* out, int64_t out_row_stride, unsigned flags,
+                          void* stream);
+
+/*
+ * bf16 products grouped by expert: out[r, i] = sum_k x[r, k] * w[e, i, k], or with transpose_w (the gradient of the rows)
+ * out[r, i] = sum_k x[r, k] * w[e, k, i], for the rows r of group e; fp32 sums, one rounding to bf16.  Groups, rows of no
+ * group and alignment as in tkq_block_scaled_gemm.  No counterpart in the reference.
+ *
+ *   x    [num_rows, k] bf16;  w  [num_experts, n, k], with transpose_w [num_experts, k, n]; rows on 16-byte boundaries
+ */
+int tkq_grouped_gemm(const void* x, int64_t x_row_stride, const void* w, int64_t w_expert_stride, int64_t w_row_stride,
+                     int transpose_w, const int32_t* expert_start, const int32_t* expert_end, int64_t num_experts,
+                     int64_t num_rows, int64_t n, int64_t k, void* out, int64_t out_row_stride, unsigned flags, void* stream);
+
+/*
+ * Gradient of each expert's weight: out[e, j, i] (+)= sum over the rows r of group e of grad[r, j] * x[r, i], fp32 sums.
+ * A group without rows gives zeros (with TKQ_ACCUMULATE: leaves its part alone).  Rows of no group are not read into any
+ * sum, whatever they hold.  No counterpart in the reference.
+ *
+ *   grad  [num_rows, n] bf16;  x  [num_rows, k] bf16; rows on 16-byte boundaries
+ *   out   [num_experts, n, k] contiguous, bf16 or fp32 (out_dtype); TKQ_ACCUMULATE needs fp32
+ */
+int tkq_grouped_gemm_wgrad(const void* grad, int64_t grad_row_stride, const void* x, int64_t x_row_stride,
+                           const int32_t* expert_start, const int32_t* expert_end, int64_t num_experts, int64_t num_rows,
+                           int64_t n, int64_t k, int out_dtype, void* out, unsigned flags, void* stream);
 
 #ifdef __cplusplus
 }

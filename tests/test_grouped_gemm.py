@@ -1,0 +1,337 @@
+"""grouped_gemm and grouped_gemm_wgrad against products in 64 bits, group by group; rows of no group; the layer they make."""
+import pytest
+import torch
+
+from product_helpers import assert_product, dequantized, int32, segments
+from test_block_scaled_gemm import quantize
+
+# group sizes: the mean decides between the tile variants, the single sizes hit their edges
+SIZES = {
+    'one': (1,), 'few': (1, 0, 2, 15, 16, 17, 0, 31, 33), 'skewed': (0, 0, 150, 1, 3), 'middle': (64, 127, 129, 0, 65, 63),
+    'large': (257, 1, 224, 300, 0, 511), 'single': (700,),
+}
+
+
+def _rows(sizes, k, device, align=1, gap=0, seed=0, first=0, spare=5):
+    """bf16 rows with NaN and infinities in all that belong to no group."""
+    start, end, used = segments(sizes, align, first, gap)
+    gen = torch.Generator().manual_seed(seed + k + sum(sizes))
+    x = torch.randn((used + spare, k), generator=gen)
+    member = torch.zeros(used + spare, dtype=torch.bool)
+    for s, e in zip(start, end):
+        member[s:e] = True
+    x[~member] = float('nan')
+    x[~member, ::3] = float('inf')
+    return x.to(torch.bfloat16).to(device), start, end, member
+
+
+def _check_groups(got, x, w, start, end, transpose=False, scale=None):
+    for e, (s, t) in enumerate(zip(start, end)):
+        if t > s:
+            assert_product(got[s:t], x[s:t], w[e].T if transpose else w[e], 1.0 if scale is None else scale[e])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', SIZES)
+@pytest.mark.parametrize('n,k', ((128, 64), (264, 200), (520, 1032)))
+@pytest.mark.parametrize('transpose', (False, True), ids=('w', 'w_t'))
+def test_bf16(cuda_device, name, n, k, transpose):
+    from tilekernels_b200 import moe
+    sizes = SIZES[name]
+    x, start, end, member = _rows(sizes, k, cuda_device, align=4 if name == 'middle' else 1, gap=3 if name == 'large' else 0)
+    gen = torch.Generator().manual_seed(n)
+    w = torch.randn((len(sizes), k, n) if transpose else (len(sizes), n, k), generator=gen).to(torch.bfloat16).to(cuda_device)
+    s, e = int32(start, cuda_device), int32(end, cuda_device)
+    got = moe.grouped_gemm(x, w, s, e, transpose_w=transpose)
+    _check_groups(got, x.cpu().double(), w.cpu().double(), start, end, transpose)
+    assert (got[~member.to(cuda_device)] == 0).all()
+    # into a given destination: rows of no group stay as they are
+    out = torch.full((x.shape[0], n + 8), 3.0, dtype=torch.bfloat16, device=cuda_device)
+    assert moe.grouped_gemm(x, w, s, e, transpose_w=transpose, out=out[:, :n]) is not None
+    assert torch.equal(out[member.to(cuda_device), :n], got[member.to(cuda_device)])
+    assert (out[~member.to(cuda_device)] == 3.0).all() and (out[:, n:] == 3.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', SIZES)
+@pytest.mark.parametrize('form', (('e4m3', (1, 128), (128, 128)), ('e4m3', (1, 32), (1, 32)), ('e2m1', (1, 32), (1, 32)),
+                                  ('nvfp4', (1, 16), (1, 16))), ids=lambda f: f'{f[0]}-{f[1][1]}')
+@pytest.mark.parametrize('n,k', ((128, 128), (328, 704)))
+def test_quantized(cuda_device, name, form, n, k):
+    from tilekernels_b200 import moe
+    fmt, xb, wb = form
+    sizes = SIZES[name]
+    x, start, end, member = _rows(sizes, k, cuda_device, gap=1 if name == 'few' else 0)
+    x[~member.to(cuda_device)] = 0
+    xq, xv, xt = quantize(x, fmt, xb)
+    if fmt != 'nvfp4':   # what the rows of no group hold does not matter: the largest scales and NaN codes there
+        data = xq[0].clone()
+        data.view(torch.uint8)[~member.to(cuda_device)] = 0x7f
+        xq = (data, xq[1])
+    gen = torch.Generator().manual_seed(n + k)
+    parts = [quantize((torch.randn((n, k), generator=gen) * 2.0 ** (i % 5)).to(torch.bfloat16).to(cuda_device), fmt, wb) for i in range(len(sizes))]
+    data = torch.stack([p[0][0].view(torch.uint8) for p in parts]).view(xq[0].dtype)
+    alpha = scale = None
+    if fmt == 'nvfp4':
+        sf = torch.stack([p[0][1].view(torch.uint8) for p in parts]).view(torch.float8_e4m3fn)
+        alpha = xt * torch.cat([p[2] for p in parts])
+        scale = alpha.double().tolist()
+    else:
+        sf = torch.stack([p[0][1].T.contiguous() for p in parts]).transpose(1, 2)
+    got = moe.grouped_gemm(xq, (data, sf), int32(start, cuda_device), int32(end, cuda_device), xb, wb, alpha=alpha)
+    _check_groups(got, xv, [p[1] for p in parts], start, end, scale=scale)
+    assert (got[~member.to(cuda_device)] == 0).all()
+
+
+@pytest.mark.gpu
+def test_scales_of_all_experts_in_one_matrix(cuda_device):
+    """The weights quantized in one call over all experts' rows."""
+    from tilekernels_b200 import moe
+    experts, n, k = 3, 256, 384
+    x, start, end, _ = _rows((40, 0, 7), k, cuda_device, spare=0)
+    gen = torch.Generator().manual_seed(1)
+    w = torch.randn((experts * n, k), generator=gen).to(torch.bfloat16).to(cuda_device)
+    xq, xv, _ = quantize(x, 'e4m3', (1, 128))
+    for block in ((128, 128), (1, 128), (32, 32)):
+        wq, wv, _ = quantize(w, 'e4m3', block)
+        got = moe.grouped_gemm(xq, (wq[0].view(experts, n, k), wq[1]), int32(start, cuda_device), int32(end, cuda_device), (1, 128), block)
+        _check_groups(got, xv, wv.view(experts, n, k), start, end)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('name', SIZES)
+@pytest.mark.parametrize('n,k', ((8, 8), (256, 128), (264, 520), (1000, 200)))
+def test_wgrad(cuda_device, name, n, k):
+    from tilekernels_b200 import moe
+    sizes = SIZES[name]
+    x, start, end, member = _rows(sizes, k, cuda_device, gap=2, first=3)
+    g, _, _, _ = _rows(sizes, n, cuda_device, gap=2, first=3, seed=1)
+    s, e = int32(start, cuda_device), int32(end, cuda_device)
+    for dtype in (torch.float32, torch.bfloat16):
+        got = moe.grouped_gemm_wgrad(g, x, s, e, out_dtype=dtype)
+        assert got.shape == (len(sizes), n, k) and got.dtype == dtype
+        for i, (a, b) in enumerate(zip(start, end)):
+            if a == b:
+                assert (got[i] == 0).all()
+            else:
+                assert_product(got[i], g[a:b].cpu().double().T, x[a:b].cpu().double().T)
+        assert torch.equal(moe.grouped_gemm_wgrad(g, x, s, e, out_dtype=dtype), got)
+    # accumulation in place; one fp32 addition more
+    before = torch.randn(got.shape, generator=torch.Generator().manual_seed(2)).to(cuda_device)
+    out = before.clone()
+    assert moe.grouped_gemm_wgrad(g, x, s, e, out=out, accumulate=True) is out
+    once = moe.grouped_gemm_wgrad(g, x, s, e)
+    assert torch.equal(out, before + once)
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences(cuda_device):
+    """The product is linear in either operand, and with small integers every sum is exact, so differences of the forward
+    product have to equal the gradients to the last bit."""
+    from tilekernels_b200 import moe
+    gen = torch.Generator().manual_seed(6)
+    sizes, n, k = (5, 0, 18, 40), 64, 32
+
+    def ints(*shape):
+        return torch.randint(-1, 2, shape, generator=gen).to(torch.bfloat16).to(cuda_device)
+
+    start, end, used = segments(sizes)
+    s, e = int32(start, cuda_device), int32(end, cuda_device)
+    x, dx, c = ints(used, k), ints(used, k), ints(used, n)
+    w, dw = ints(len(sizes), n, k), ints(len(sizes), n, k)
+
+    def f(x, w):
+        return (moe.grouped_gemm(x, w, s, e).double() * c.double()).sum().item()
+
+    grad_x = moe.grouped_gemm(c, w, s, e, transpose_w=True).double()
+    grad_w = moe.grouped_gemm_wgrad(c, x, s, e).double()
+    assert f(x + dx, w) - f(x - dx, w) == 2 * (grad_x * dx.double()).sum().item()
+    assert f(x, w + dw) - f(x, w - dw) == 2 * (grad_w * dw.double()).sum().item()
+
+
+@pytest.mark.gpu
+def test_bounds_outside_the_rows_are_clamped(cuda_device):
+    from tilekernels_b200 import moe
+    x, _, _, _ = _rows((20,), 64, cuda_device, spare=0)
+    w = torch.ones((3, 32, 64), dtype=torch.bfloat16, device=cuda_device)
+    s, e = int32([-5, 8, 30], cuda_device), int32([8, 1000, 7], cuda_device)
+    got = moe.grouped_gemm(x, w, s, e)
+    _check_groups(got, x.cpu().double(), w.cpu().double(), [0, 8], [8, 20])
+    dw = moe.grouped_gemm_wgrad(x, x, s, e)
+    assert_product(dw[0], x[:8].cpu().double().T, x[:8].cpu().double().T)
+    assert_product(dw[1], x[8:].cpu().double().T, x[8:].cpu().double().T)
+    assert (dw[2] == 0).all()
+
+
+@pytest.mark.gpu
+def test_strided_operands(cuda_device):
+    from tilekernels_b200 import moe
+    sizes, n, k = (33, 0, 90), 136, 72
+    start, end, used = segments(sizes)
+    gen = torch.Generator().manual_seed(8)
+    xs = torch.randn((used, k + 24), generator=gen).to(torch.bfloat16).to(cuda_device)
+    ws = torch.randn((3, n + 5, k + 16), generator=gen).to(torch.bfloat16).to(cuda_device)
+    x, w = xs[:, 8:8 + k], ws[:, 2:2 + n, 8:8 + k]
+    s, e = int32(start, cuda_device), int32(end, cuda_device)
+    _check_groups(moe.grouped_gemm(x, w, s, e), x.cpu().double(), w.cpu().double(), start, end)
+    got = moe.grouped_gemm_wgrad(xs[:, 16:16 + 40], x, s, e)
+    assert_product(got[2], xs[start[2]:end[2], 16:56].cpu().double().T, x[start[2]:end[2]].cpu().double().T)
+
+
+@pytest.mark.gpu
+def test_many_experts(cuda_device):
+    from tilekernels_b200 import moe
+    gen = torch.Generator().manual_seed(11)
+    sizes = torch.randint(0, 4, (1024,), generator=gen).tolist()
+    x, start, end, _ = _rows(sizes, 64, cuda_device)
+    w = torch.randn((1024, 16, 64), generator=gen).to(torch.bfloat16).to(cuda_device)
+    s, e = int32(start, cuda_device), int32(end, cuda_device)
+    got = moe.grouped_gemm(x, w, s, e)
+    _check_groups(got, x.cpu().double(), w.cpu().double(), start, end)
+    dw = moe.grouped_gemm_wgrad(x, x, s, e)
+    for i in range(0, 1024, 97):
+        if sizes[i]:
+            rows = x[start[i]:end[i]].cpu().double()
+            assert_product(dw[i], rows.T, rows.T)
+
+
+@pytest.mark.gpu
+def test_no_rows(cuda_device):
+    from tilekernels_b200 import moe
+    w = torch.ones((2, 16, 64), dtype=torch.bfloat16, device=cuda_device)
+    zero = int32([0, 0], cuda_device)
+    empty = torch.empty((0, 64), dtype=torch.bfloat16, device=cuda_device)
+    assert moe.grouped_gemm(empty, w, zero, zero).shape == (0, 16)
+    assert (moe.grouped_gemm_wgrad(empty[:, :16], empty, zero, zero) == 0).all()
+    out = torch.full((2, 16, 64), 2.0, device=cuda_device)
+    moe.grouped_gemm_wgrad(empty[:, :16], empty, zero, zero, out=out, accumulate=True)
+    assert (out == 2.0).all()
+    # rows, but all of them of no expert
+    x = torch.full((9, 64), float('nan'), dtype=torch.bfloat16, device=cuda_device)
+    assert (moe.grouped_gemm(x, w, zero, zero) == 0).all()
+    assert (moe.grouped_gemm_wgrad(x[:, :16], x, zero, zero) == 0).all()
+
+
+@pytest.mark.gpu
+def test_graph_follows_the_group_bounds(cuda_device):
+    """Captured once, replayed with other rows and other segments: nothing about the groups is fixed at capture."""
+    from tilekernels_b200 import moe
+    n, k, rows = 200, 136, 400
+    gen = torch.Generator().manual_seed(13)
+    w = torch.randn((4, n, k), generator=gen).to(torch.bfloat16).to(cuda_device)
+    x = torch.zeros((rows, k), dtype=torch.bfloat16, device=cuda_device)
+    s, e = int32([0] * 4, cuda_device), int32([0] * 4, cuda_device)
+    main = torch.zeros((4, n, k), device=cuda_device)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            y = moe.grouped_gemm(x, w, s, e)
+            dx = moe.grouped_gemm(y, w, s, e, transpose_w=True)
+            moe.grouped_gemm_wgrad(y, x, s, e, out=main, accumulate=True)
+    for sizes in ((100, 100, 100, 100), (0, 399, 0, 1), (7, 0, 0, 0)):
+        start, end, _ = segments(sizes)
+        new = torch.randn((rows, k), generator=gen).to(torch.bfloat16).to(cuda_device)
+        with torch.cuda.stream(stream):
+            x.copy_(new)
+            s.copy_(int32(start, cuda_device))
+            e.copy_(int32(end, cuda_device))
+            main.zero_()
+            graph.replay()
+        torch.cuda.synchronize()
+        _check_groups(y, x.cpu().double(), w.cpu().double(), start, end)
+        _check_groups(dx, y.cpu().double(), w.cpu().double(), start, end, transpose=True)
+        for i, (a, b) in enumerate(zip(start, end)):
+            if a < b:
+                assert_product(main[i], y[a:b].cpu().double().T, x[a:b].cpu().double().T)
+        assert (y[sum(sizes):] == 0).all()
+
+
+@pytest.mark.gpu
+def test_expert_layer(cuda_device):
+    """The way of a batch through quantized experts and back: expansion, up-projection, activation and cast, down-projection;
+    then both products' gradients in bf16.  Every step is compared with 64 bits on the inputs it was given."""
+    from tilekernels_b200 import moe, quant
+    from test_block_scaled_gemm import PACKED
+    gen = torch.Generator().manual_seed(21)
+    tokens, hidden, inter, experts, topk, align = 60, 512, 256, 4, 2, 16
+    x = torch.randn((tokens, hidden), generator=gen).to(torch.bfloat16).to(cuda_device)
+    choice = torch.stack([torch.randperm(experts, generator=gen)[:topk] for _ in range(tokens)])
+    order, start, end, at = [], [], [], 0
+    for e in range(experts):
+        mine = (choice == e).nonzero().tolist()
+        start.append(at)
+        end.append(at + len(mine))
+        order.append(mine)
+        at = -(-end[-1] // align) * align
+    t2p = torch.full((tokens, topk), -1, dtype=torch.int32)
+    p2e = torch.full((at,), -1, dtype=torch.int32)
+    for e in range(experts):
+        for i, (t, j) in enumerate(order[e]):
+            t2p[t, j] = start[e] + i
+            p2e[start[e] + i] = e
+    t2p, p2e = t2p.to(cuda_device), p2e.to(cuda_device)
+    s, e = int32(start, cuda_device), int32(end, cuda_device)
+    w1 = (torch.randn((experts, 2 * inter, hidden), generator=gen) * 0.05).to(torch.bfloat16).to(cuda_device)
+    w2 = (torch.randn((experts, hidden, inter), generator=gen) * 0.05).to(torch.bfloat16).to(cuda_device)
+    w1q = quant.per_block_cast(w1.view(-1, hidden), 'e4m3', (128, 128), **PACKED)
+    w2q = quant.per_block_cast(w2.view(-1, inter), 'e4m3', (128, 128), **PACKED)
+    w1v = dequantized(*w1q, (128, 128)).view(w1.shape)
+    w2v = dequantized(*w2q, (128, 128)).view(w2.shape)
+
+    q, sf = quant.per_token_cast(x, 'e4m3', 128, None, True, True, True)
+    xq = moe.expand_to_fused_with_sf((q, sf.contiguous()), 128, t2p, p2e, True)
+    up = moe.grouped_gemm(xq, (w1q[0].view(w1.shape), w1q[1]), s, e, (1, 128), (128, 128))
+    _check_groups(up, dequantized(*xq, (1, 128)), w1v, start, end)
+    act = quant.swiglu_forward_and_per_token_cast(up, 'e4m3', 128, pos_to_expert=p2e, **PACKED)
+    down = moe.grouped_gemm(act, (w2q[0].view(w2.shape), w2q[1]), s, e, (1, 128), (128, 128))
+    _check_groups(down, dequantized(*act, (1, 128)), w2v, start, end)
+    assert (down[p2e < 0] == 0).all()
+
+    xe = moe.expand_to_fused(x, t2p, p2e)
+    d_up = torch.randn(up.shape, generator=gen).to(torch.bfloat16).to(cuda_device)
+    dx = moe.grouped_gemm(d_up, w1, s, e, transpose_w=True)
+    dw1 = moe.grouped_gemm_wgrad(d_up, xe, s, e)
+    _check_groups(dx, d_up.cpu().double(), w1.cpu().double(), start, end, transpose=True)
+    for i in range(experts):
+        rows = slice(start[i], end[i])
+        assert_product(dw1[i], d_up[rows].cpu().double().T, xe[rows].cpu().double().T)
+
+
+@pytest.mark.gpu
+def test_refusals(cuda_device):
+    from tilekernels_b200 import moe
+    x = torch.zeros((8, 64), dtype=torch.bfloat16, device=cuda_device)
+    w = torch.zeros((2, 32, 64), dtype=torch.bfloat16, device=cuda_device)
+    s, e = int32([0, 4], cuda_device), int32([4, 8], cuda_device)
+    for args, kw in (
+        ((x.float(), w, s, e), {}), ((x, w.half(), s, e), {}), ((x[:, :32], w, s, e), {}), ((x, w, s[:1], e), {}), ((x, w, s.long(), e), {}),
+        ((x, w, s.cpu(), e), {}), ((x, w[0], s, e), {}), ((x, w, s, e), dict(alpha=torch.ones(1, device=cuda_device))),
+        ((x, w, s, e), dict(x_block_size=(1, 128))), ((x.T, w, s, e), {}), ((x, w, s, e), dict(transpose_w=True)),
+        ((x, w, s, e), dict(out=torch.empty((8, 33), dtype=torch.bfloat16, device=cuda_device))),
+        (((x.view(torch.int8), s), (w.view(torch.int8), s), s, e), dict(x_block_size=(1, 32), w_block_size=(1, 32), transpose_w=True)),
+    ):
+        with pytest.raises(AssertionError):
+            moe.grouped_gemm(*args, **kw)
+    with pytest.raises(RuntimeError, match='16-byte'):
+        moe.grouped_gemm(torch.zeros((8, 68), dtype=torch.bfloat16, device=cuda_device)[:, :64], w, s, e)
+    with pytest.raises(RuntimeError, match='1024'):
+        many = torch.zeros(1025, dtype=torch.int32, device=cuda_device)
+        moe.grouped_gemm_wgrad(x, x, many, many)
+    for args, kw in (
+        ((x.float(), x, s, e), {}), ((x[:4], x, s, e), {}), ((x, x, s, e), dict(out_dtype=torch.float16)), ((x, x, s, e), dict(accumulate=True)),
+        ((x, x, s, e), dict(out=torch.empty((2, 64, 64), dtype=torch.bfloat16, device=cuda_device))),
+        ((x, x, s, e), dict(out_dtype=torch.bfloat16, accumulate=True, out=torch.empty((2, 64, 64), dtype=torch.bfloat16, device=cuda_device))),
+    ):
+        with pytest.raises(AssertionError):
+            moe.grouped_gemm_wgrad(*args, **kw)
+
+
+def test_cpu_tensors_are_refused():
+    from tilekernels_b200 import moe
+    x, w = torch.zeros((8, 64), dtype=torch.bfloat16), torch.zeros((2, 32, 64), dtype=torch.bfloat16)
+    bounds = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(AssertionError):
+        moe.grouped_gemm(x, w, bounds, bounds)
+    with pytest.raises(AssertionError):
+        moe.grouped_gemm_wgrad(x, x, bounds, bounds)

@@ -10,6 +10,8 @@ LIB_PATH = os.environ.get('TKQ_LIB_PATH') or os.path.join(_HERE, 'lib', 'libtkqu
 DT_BF16, DT_FP32 = 0, 1
 FMT_E4M3, FMT_E2M1, FMT_E5M6 = 0, 1, 2
 ROUND_SF, SF_COL_MAJOR, SF_UE8M0, SF_ONLY, CAST_ONLY, EXACT_CODES = 1, 2, 4, 8, 16, 32
+ZERO_GAPS, ACCUMULATE = 64, 128
+SFMT_UE8M0, SFMT_E4M3 = 0, 1
 
 _vp, _i64, _int, _uint, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_uint, ctypes.c_float
 
@@ -34,6 +36,12 @@ SIGNATURES = {
     'tkq_swiglu_backward_and_per_token_cast': [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _uint,
                                                _vp, _vp, _vp, _vp, _vp, _vp],
     'tkq_expand_to_fused': [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _uint, _vp, _vp, _i64, _vp],
+    'tkq_per_token_cast_nvfp4': [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp],
+    'tkq_cast_back_nvfp4': [_vp, _vp, _vp, _i64, _i64, _int, _vp, _vp],
+    'tkq_block_scaled_gemm': [_vp, _i64, _vp, _i64, _i64, _int, _int, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _int, _int, _int, _int,
+                              _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _uint, _vp],
+    'tkq_grouped_gemm': [_vp, _i64, _vp, _i64, _i64, _int, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _uint, _vp],
+    'tkq_grouped_gemm_wgrad': [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp, _uint, _vp],
 }
 
 _lib = None

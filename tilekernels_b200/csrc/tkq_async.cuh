@@ -97,5 +97,6 @@ __device__ __forceinline__ void tma_load_tile(void* smem_dst, const CUtensorMap*
 int tile_wait_flag();
 int row_wait_flag();
 int swiglu_wait_flag();
+int gemm_wait_flag();
 
 }  // namespace tkq

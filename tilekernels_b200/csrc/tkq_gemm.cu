@@ -1,0 +1,232 @@
+// C entry points of the matrix products: argument checks, tensor maps, choice of the tile variant, launch.
+#include <cudaTypedefs.h>
+
+#include "tkq_gemm.cuh"
+
+namespace tkq {
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();  // tkq_tile.cu
+
+int gemm_wait_flag() {
+    unsigned int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_gemm_wait_failed, sizeof(v)) != cudaSuccess) return -1;
+    if (v) {
+        const unsigned int zero = 0;
+        if (cudaMemcpyToSymbol(g_gemm_wait_failed, &zero, sizeof(zero)) != cudaSuccess) return -1;
+    }
+    return v ? 1 : 0;
+}
+
+// One operand as a three-dimensional tensor (inner axis, rows, groups); strides in bytes.
+struct Operand {
+    const void* base;
+    int64_t inner, rows, groups;
+    int64_t row_bytes, group_bytes;
+    bool bf16;
+};
+
+static int encode(CUtensorMap* map, const Operand& o, uint32_t box_inner, uint32_t box_rows) {
+    auto fn = tensor_map_encoder();
+    if (fn == nullptr) return set_error(TKQ_E_UNSUPPORTED, "cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(o.inner), static_cast<cuuint64_t>(o.rows), static_cast<cuuint64_t>(o.groups)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.row_bytes), static_cast<cuuint64_t>(o.group_bytes)};
+    const cuuint32_t box[3] = {box_inner, box_rows, 1};
+    const cuuint32_t steps[3] = {1, 1, 1};
+    const CUresult r = fn(map, o.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(o.base), dims,
+                          strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(TKQ_E_UNSUPPORTED, "cuTensorMapEncodeTiled rejected an operand (alignment or size)");
+    return 0;
+}
+
+// Strides a tensor map accepts: multiples of 16 bytes.  The stride of an axis of length one is never used, so any stands in.
+static bool fix_strides(Operand& o) {
+    const int64_t tight = (o.inner * (o.bf16 ? 2 : 1) + 15) / 16 * 16;
+    if (o.rows == 1) o.row_bytes = tight;
+    if (o.groups == 1) o.group_bytes = o.row_bytes * o.rows;
+    return o.row_bytes % 16 == 0 && o.group_bytes % 16 == 0 && o.row_bytes > 0 && o.group_bytes > 0 && aligned16(o.base);
+}
+
+template <class C>
+static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const char* what, cudaStream_t stream) {
+    alignas(64) CUtensorMap map_a, map_b;
+    if (int rc = encode(&map_a, a, C::A_MN ? 64 : C::kElems, C::A_MN ? 64 : 128)) return rc;
+    if (int rc = encode(&map_b, b, C::WGRAD ? 64 : C::kElems, C::WGRAD ? 64 : C::kBRows)) return rc;
+    p.i_tiles = (p.i_size + 128 * C::CG - 1) / (128 * C::CG);
+    const int64_t j_tiles = C::WGRAD ? int64_t{p.groups} * ((p.j_size + C::NMAX - 1) / C::NMAX) : int64_t{p.rows} / C::NMAX + p.groups;
+    if (j_tiles * p.i_tiles >= (int64_t{1} << 31)) return set_error(TKQ_E_UNSUPPORTED, "matrix product: more than 2^31 tiles");
+    const int64_t units = std::min<int64_t>(j_tiles * p.i_tiles, device_sm_count() / C::CG);
+    const int smem = static_cast<int>(1024 + C::kStages * C::kStageBytes + 4 * (3 * p.groups + 1));
+    auto kernel = gemm_kernel<C>;
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(units * C::CG));
+    config.blockDim = dim3(kGemmThreads);
+    config.dynamicSmemBytes = static_cast<size_t>(smem);
+    config.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = C::CG;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = C::CG > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, map_a, map_b, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(static_cast<int>(e), cudaGetErrorString(e));
+    }
+    return check_launch(what);
+}
+
+// Tile variant by the mean number of rows per group.
+template <int KIND, int NLARGE, bool A_MN>
+static int launch_rows(const Operand& a, const Operand& b, const GemmParams& p, const char* what, cudaStream_t stream) {
+    const int64_t mean = p.rows / p.groups;
+    if (mean <= 32) return launch_gemm<GemmConfig<KIND, 1, 32, false, A_MN>>(a, b, p, what, stream);
+    if (mean <= 128) return launch_gemm<GemmConfig<KIND, 1, 128, false, A_MN>>(a, b, p, what, stream);
+    return launch_gemm<GemmConfig<KIND, 2, NLARGE, false, A_MN>>(a, b, p, what, stream);
+}
+
+static int check_sizes(int64_t num_experts, int64_t num_rows, int64_t n, int64_t k) {
+    if (num_experts <= 0 || num_rows < 0 || n <= 0 || k <= 0) return set_error(TKQ_E_BAD_ARG, "matrix product: bad size");
+    if (num_experts > kMaxGroups) return set_error(TKQ_E_UNSUPPORTED, "matrix product: more than 1024 groups");
+    if (num_rows >= (int64_t{1} << 30) || n >= (int64_t{1} << 30) || k >= (int64_t{1} << 30))
+        return set_error(TKQ_E_UNSUPPORTED, "matrix product: an axis of 2^30 or more");
+    return 0;
+}
+
+}  // namespace tkq
+
+using namespace tkq;
+
+extern "C" int tkq_block_scaled_gemm(const void* x, int64_t x_row_stride, const void* x_sf, int64_t x_sf_row_stride, int64_t x_sf_k_stride,
+                                     int x_block_m, int x_block_k, const void* w, int64_t w_expert_stride, int64_t w_row_stride, const void* w_sf,
+                                     int64_t w_sf_expert_stride, int64_t w_sf_row_stride, int64_t w_sf_k_stride, int w_block_m, int w_block_k,
+                                     int fmt, int sf_fmt, const int32_t* expert_start, const int32_t* expert_end, int64_t num_experts,
+                                     int64_t num_rows, int64_t n, int64_t k, const float* alpha, int64_t alpha_stride, void* out,
+                                     int64_t out_row_stride, unsigned flags, void* stream) {
+    if (int rc = check_sizes(num_experts, num_rows, n, k)) return rc;
+    if ((fmt != TKQ_FMT_E4M3 && fmt != TKQ_FMT_E2M1) || (sf_fmt != TKQ_SFMT_UE8M0 && sf_fmt != TKQ_SFMT_E4M3))
+        return set_error(TKQ_E_BAD_ARG, "block_scaled_gemm: unknown format");
+    if (flags & ~static_cast<unsigned>(TKQ_ZERO_GAPS)) return set_error(TKQ_E_UNSUPPORTED, "block_scaled_gemm: only TKQ_ZERO_GAPS applies");
+    if (num_rows == 0) return 0;
+    if (x == nullptr || x_sf == nullptr || w == nullptr || w_sf == nullptr || out == nullptr || (expert_start == nullptr) != (expert_end == nullptr) ||
+        (expert_start == nullptr && num_experts != 1))
+        return set_error(TKQ_E_BAD_ARG, "block_scaled_gemm: null pointer");
+    const bool fp8 = fmt == TKQ_FMT_E4M3, nv = sf_fmt == TKQ_SFMT_E4M3;
+    auto shift_of = [](int v) { return v == 1 ? 0 : v == 32 ? 5 : v == 128 ? 7 : -1; };
+    const int xs = shift_of(x_block_m), ws = shift_of(w_block_m);
+    bool group_ok;
+    if (fp8) group_ok = !nv && (x_block_k == 32 || x_block_k == 128) && (w_block_k == 32 || w_block_k == 128);
+    else group_ok = x_block_k == (nv ? 16 : 32) && w_block_k == (nv ? 16 : 32);
+    if (!group_ok || xs < 0 || ws < 0)
+        return set_error(TKQ_E_UNSUPPORTED, "block_scaled_gemm: scale blocks are 1, 32 or 128 rows by 32 or 128 (e4m3), 32 (e2m1) or 16 (e2m1 with e4m3 scales) values");
+    if (k % (fp8 ? 32 : 64) != 0) return set_error(TKQ_E_UNSUPPORTED, "block_scaled_gemm: k must be a multiple of 32 (e4m3) or 64 (e2m1)");
+    const int64_t per_byte = fp8 ? 1 : 2;
+    if (x_row_stride % per_byte || w_row_stride % per_byte || w_expert_stride % per_byte)
+        return set_error(TKQ_E_ALIGNMENT, "block_scaled_gemm: strides of packed e2m1 data are even");
+    Operand a{w, k / per_byte, n, num_experts, w_row_stride / per_byte, w_expert_stride / per_byte, false};
+    Operand b{x, k / per_byte, num_rows, 1, x_row_stride / per_byte, 0, false};
+    if (!fix_strides(a) || !fix_strides(b) || (reinterpret_cast<uintptr_t>(x_sf) & 3u) || (reinterpret_cast<uintptr_t>(w_sf) & 3u) ||
+        (reinterpret_cast<uintptr_t>(out) & 1u))
+        return set_error(TKQ_E_ALIGNMENT, "block_scaled_gemm: data rows on 16-byte boundaries, scales on 4-byte boundaries");
+    GemmParams p{};
+    p.start = expert_start;
+    p.end = expert_end;
+    p.alpha = alpha;
+    p.alpha_stride = static_cast<uint32_t>(alpha_stride);
+    p.out = out;
+    p.out_stride = out_row_stride;
+    p.groups = static_cast<uint32_t>(num_experts);
+    p.rows = static_cast<uint32_t>(num_rows);
+    p.i_size = static_cast<uint32_t>(n);
+    const int64_t row_bytes = k / per_byte;
+    p.k_blocks = static_cast<uint32_t>((row_bytes + 127) / 128);
+    p.last_units = static_cast<uint32_t>((row_bytes - (int64_t{p.k_blocks} - 1) * 128) / 32);
+    p.zero_gaps = (flags & TKQ_ZERO_GAPS) ? 1 : 0;
+    p.pair_stores = n % 2 == 0 && out_row_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
+    auto view = [&](const void* sf, int64_t e, int64_t r, int64_t q, int shift, int block_k) {
+        ScaleView v{};
+        v.base = static_cast<const uint32_t*>(sf);
+        v.group_stride = e;
+        v.row_stride = r;
+        v.k_stride = q;
+        v.row_shift = static_cast<uint32_t>(shift);
+        v.words = static_cast<uint32_t>((k + 4 * block_k - 1) / (4 * block_k));
+        v.k_shift = block_k == 128 ? 2 : 0;
+        v.vec = q == 1 && r % 4 == 0 && e % 4 == 0 && aligned16(sf);
+        return v;
+    };
+    p.sfa = view(w_sf, w_sf_expert_stride, w_sf_row_stride, w_sf_k_stride, ws, w_block_k);
+    p.sfb = view(x_sf, 0, x_sf_row_stride, x_sf_k_stride, xs, x_block_k);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (fp8) return launch_rows<kKindMxf8, 224, false>(a, b, p, "block_scaled_gemm", s);
+    if (!nv) return launch_rows<kKindMxf4, 224, false>(a, b, p, "block_scaled_gemm", s);
+    return launch_rows<kKindNvf4, 192, false>(a, b, p, "block_scaled_gemm", s);
+}
+
+extern "C" int tkq_grouped_gemm(const void* x, int64_t x_row_stride, const void* w, int64_t w_expert_stride, int64_t w_row_stride, int transpose_w,
+                                const int32_t* expert_start, const int32_t* expert_end, int64_t num_experts, int64_t num_rows, int64_t n,
+                                int64_t k, void* out, int64_t out_row_stride, unsigned flags, void* stream) {
+    if (int rc = check_sizes(num_experts, num_rows, n, k)) return rc;
+    if (flags & ~static_cast<unsigned>(TKQ_ZERO_GAPS)) return set_error(TKQ_E_UNSUPPORTED, "grouped_gemm: only TKQ_ZERO_GAPS applies");
+    if (num_rows == 0) return 0;
+    if (x == nullptr || w == nullptr || out == nullptr || expert_start == nullptr || expert_end == nullptr)
+        return set_error(TKQ_E_BAD_ARG, "grouped_gemm: null pointer");
+    Operand a{w, transpose_w ? n : k, transpose_w ? k : n, num_experts, w_row_stride * 2, w_expert_stride * 2, true};
+    Operand b{x, k, num_rows, 1, x_row_stride * 2, 0, true};
+    if (!fix_strides(a) || !fix_strides(b) || (reinterpret_cast<uintptr_t>(out) & 1u))
+        return set_error(TKQ_E_ALIGNMENT, "grouped_gemm: rows of x and w on 16-byte boundaries");
+    GemmParams p{};
+    p.start = expert_start;
+    p.end = expert_end;
+    p.out = out;
+    p.out_stride = out_row_stride;
+    p.groups = static_cast<uint32_t>(num_experts);
+    p.rows = static_cast<uint32_t>(num_rows);
+    p.i_size = static_cast<uint32_t>(n);
+    p.k_blocks = static_cast<uint32_t>((k + 63) / 64);
+    p.last_units = static_cast<uint32_t>((k - (int64_t{p.k_blocks} - 1) * 64 + 15) / 16);
+    p.zero_gaps = (flags & TKQ_ZERO_GAPS) ? 1 : 0;
+    p.pair_stores = n % 2 == 0 && out_row_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (transpose_w) return launch_rows<kKindBf16, 256, true>(a, b, p, "grouped_gemm", s);
+    return launch_rows<kKindBf16, 256, false>(a, b, p, "grouped_gemm", s);
+}
+
+extern "C" int tkq_grouped_gemm_wgrad(const void* grad, int64_t grad_row_stride, const void* x, int64_t x_row_stride, const int32_t* expert_start,
+                                      const int32_t* expert_end, int64_t num_experts, int64_t num_rows, int64_t n, int64_t k, int out_dtype,
+                                      void* out, unsigned flags, void* stream) {
+    if (int rc = check_sizes(num_experts, num_rows, n, k)) return rc;
+    if (out_dtype != TKQ_DT_BF16 && out_dtype != TKQ_DT_FP32) return set_error(TKQ_E_BAD_ARG, "grouped_gemm_wgrad: unknown output type");
+    if (flags & ~static_cast<unsigned>(TKQ_ACCUMULATE)) return set_error(TKQ_E_UNSUPPORTED, "grouped_gemm_wgrad: only TKQ_ACCUMULATE applies");
+    if ((flags & TKQ_ACCUMULATE) && out_dtype != TKQ_DT_FP32)
+        return set_error(TKQ_E_UNSUPPORTED, "grouped_gemm_wgrad: accumulation needs a float32 output");
+    if (out == nullptr || expert_start == nullptr || expert_end == nullptr || (num_rows > 0 && (grad == nullptr || x == nullptr)))
+        return set_error(TKQ_E_BAD_ARG, "grouped_gemm_wgrad: null pointer");
+    if (num_rows == 0) {  // every group is empty: gradients of zero
+        if (flags & TKQ_ACCUMULATE) return 0;
+        const cudaError_t e = cudaMemsetAsync(out, 0, static_cast<size_t>(num_experts * n * k) * (out_dtype == TKQ_DT_FP32 ? 4 : 2),
+                                              static_cast<cudaStream_t>(stream));
+        return e == cudaSuccess ? 0 : set_error(static_cast<int>(e), "grouped_gemm_wgrad: memset failed");
+    }
+    Operand a{x, k, num_rows, 1, x_row_stride * 2, 0, true};
+    Operand b{grad, n, num_rows, 1, grad_row_stride * 2, 0, true};
+    if (!fix_strides(a) || !fix_strides(b) || (reinterpret_cast<uintptr_t>(out) & (out_dtype == TKQ_DT_FP32 ? 3u : 1u)))
+        return set_error(TKQ_E_ALIGNMENT, "grouped_gemm_wgrad: rows of grad and x on 16-byte boundaries");
+    GemmParams p{};
+    p.start = expert_start;
+    p.end = expert_end;
+    p.out = out;
+    p.out_stride = k;
+    p.out_group_stride = n * k;
+    p.groups = static_cast<uint32_t>(num_experts);
+    p.rows = static_cast<uint32_t>(num_rows);
+    p.i_size = static_cast<uint32_t>(k);
+    p.j_size = static_cast<uint32_t>(n);
+    p.out_f32 = out_dtype == TKQ_DT_FP32;
+    p.accumulate = (flags & TKQ_ACCUMULATE) ? 1 : 0;
+    p.pair_stores = k % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true>>(a, b, p, "grouped_gemm_wgrad", s);
+}

@@ -1023,7 +1023,7 @@ __global__ void __launch_bounds__(kTileThreads, kLosslessBlocksPerSm) per_block_
 }
 
 // cuTensorMapEncodeTiled through the runtime's driver entry-point lookup (no link against libcuda).
-static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -1263,9 +1263,9 @@ static int lossless_violation_flag() {
 }
 
 extern "C" int tkq_device_error(void) {
-    const int a = tile_wait_flag(), b = row_wait_flag(), c = swiglu_wait_flag(), d = lossless_violation_flag();
-    if (a < 0 || b < 0 || c < 0 || d < 0) return -1;
-    return ((a | b | c) ? TKQ_DEVICE_WAIT_TIMEOUT : 0) | (d ? TKQ_DEVICE_LOSSLESS_RANGE : 0);
+    const int a = tile_wait_flag(), b = row_wait_flag(), c = swiglu_wait_flag(), d = lossless_violation_flag(), e = gemm_wait_flag();
+    if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0) return -1;
+    return ((a | b | c | e) ? TKQ_DEVICE_WAIT_TIMEOUT : 0) | (d ? TKQ_DEVICE_LOSSLESS_RANGE : 0);
 }
 
 namespace tkq {

@@ -6,3 +6,4 @@ from .. import _lib as _lib_module
 _lib_module.lib()  # fail at import when the CUDA library is missing
 
 from .expand_to_fused_kernel import expand_to_fused, expand_to_fused_with_sf  # noqa: E402
+from .grouped_gemm_kernel import grouped_gemm, grouped_gemm_wgrad  # noqa: E402

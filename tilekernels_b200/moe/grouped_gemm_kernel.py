@@ -1,0 +1,127 @@
+"""grouped_gemm, grouped_gemm_wgrad: products of rows sorted by expert with each expert's weight, and their gradients.  The
+reference lays rows out for such products (expand_to_fused) and leaves the products to another library."""
+from typing import Optional, Union
+
+import torch
+
+from .. import _lib
+from ..quant.block_scaled_gemm_kernel import check_out, launch_block_scaled_gemm, scaled_operand
+from ..quant.common import DTYPE_TO_ENUM, current_stream_ptr, device_guard
+from ..quant.types import QuantTensor
+
+
+def _check_groups(expert_start: torch.Tensor, expert_end: torch.Tensor, num_experts: int, device: torch.device) -> None:
+    for t in (expert_start, expert_end):
+        assert t.dtype == torch.int32 and t.device == device and t.is_contiguous() and tuple(t.shape) == (num_experts,)
+
+
+def _check_matrix(x: torch.Tensor, dim: int) -> None:
+    assert x.dtype == torch.bfloat16 and x.is_cuda and x.dim() == dim
+    assert x.shape[-1] <= 1 or x.stride(-1) == 1
+
+
+def grouped_gemm(
+    x: Union[torch.Tensor, QuantTensor],
+    w: Union[torch.Tensor, QuantTensor],
+    expert_start: torch.Tensor,
+    expert_end: torch.Tensor,
+    x_block_size: Optional[tuple[int, int]] = None,
+    w_block_size: Optional[tuple[int, int]] = None,
+    alpha: Optional[torch.Tensor] = None,
+    transpose_w: bool = False,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """out[r] = x[r] @ w[e].T for the rows r of every expert e, expert_start[e] <= r < expert_end[e].
+
+    Args:
+        x: (num_rows, k) bfloat16, or a quantized pair in a form of quant.block_scaled_gemm.
+        w: (num_experts, n, k) bfloat16; with transpose_w (num_experts, k, n), which with the gradient of the output as x
+            gives the gradient of the input.  Or a quantized pair: data (num_experts, n, k), scales
+            (num_experts, blocks of rows, words) or, for whole blocks, one matrix of all experts' rows.
+        expert_start, expert_end: int32 (num_experts,), ascending; segments may be empty, of any length and alignment, and
+            need not touch.  At most 1024 experts.
+        x_block_size, w_block_size: (rows, values) per scale of quantized operands, as in quant.block_scaled_gemm.
+        alpha: optional fp32 tensor with one factor for all or one per expert (quantized operands).
+        out: optional (num_rows, n) bfloat16 destination with unit column stride.  Rows of no expert are left as they
+            are; without `out` they are zero.
+
+    Rows of bfloat16 operands start on 16-byte boundaries (k, and n with transpose_w, multiples of 8 when contiguous).
+
+    Returns: (num_rows, n) bfloat16; fp32 sums, one rounding.
+    """
+    flags = _lib.ZERO_GAPS if out is None else 0
+    if isinstance(x, tuple):
+        assert isinstance(w, tuple) and x_block_size is not None and w_block_size is not None
+        assert not transpose_w, 'quantized weights are scaled along k: quantize the transposed weight instead'
+        num_experts = w[0].shape[0]
+        xo, wo = scaled_operand(x, x_block_size, None), scaled_operand(w, w_block_size, num_experts)
+        num_rows, n, device = xo['rows'], wo['rows'], xo['data'].device
+        assert num_experts >= 1 and xo['k'] > 0 and xo['k'] == wo['k'], f"inner sizes differ: {xo['k']} and {wo['k']}"
+        assert wo['data'].device == device
+    else:
+        assert isinstance(w, torch.Tensor) and x_block_size is None and w_block_size is None and alpha is None
+        _check_matrix(x, 2)
+        _check_matrix(w, 3)
+        assert w.device == x.device
+        num_experts, n, k = (w.shape[0], w.shape[2], w.shape[1]) if transpose_w else w.shape
+        num_rows, device = x.shape[0], x.device
+        assert num_experts >= 1 and k > 0 and x.shape[1] == k, f'inner sizes differ: {x.shape[1]} and {k}'
+    _check_groups(expert_start, expert_end, num_experts, device)
+    if out is None:
+        out = torch.empty((num_rows, n), dtype=torch.bfloat16, device=device)
+    else:
+        check_out(out, (num_rows, n), torch.bfloat16, device)
+    if isinstance(x, tuple):
+        launch_block_scaled_gemm(xo, wo, expert_start, expert_end, num_experts, alpha, out, flags)
+    elif num_rows > 0 and n > 0:
+        with device_guard(device):
+            rc = _lib.lib().tkq_grouped_gemm(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w.stride(1), int(transpose_w),
+                                             expert_start.data_ptr(), expert_end.data_ptr(), num_experts, num_rows, n, k, out.data_ptr(),
+                                             out.stride(0), flags, current_stream_ptr(device))
+        _lib.check(rc, 'tkq_grouped_gemm')
+    return out
+
+
+def grouped_gemm_wgrad(
+    grad: torch.Tensor,
+    x: torch.Tensor,
+    expert_start: torch.Tensor,
+    expert_end: torch.Tensor,
+    out_dtype: torch.dtype = torch.float32,
+    out: Optional[torch.Tensor] = None,
+    accumulate: bool = False,
+) -> torch.Tensor:
+    """The gradient of grouped_gemm's weight: dw[e] = grad[rows of e].T @ x[rows of e].
+
+    Args:
+        grad: (num_rows, n) bfloat16, gradient of the output.
+        x: (num_rows, k) bfloat16, the input.  Rows of both start on 16-byte boundaries.
+        expert_start, expert_end: as in grouped_gemm; rows of no expert are not read into any sum.
+        out_dtype: torch.float32 or torch.bfloat16.
+        out: optional contiguous (num_experts, n, k) destination of out_dtype.
+        accumulate: add to `out` (float32 only); experts without rows leave their part alone.
+
+    Returns: (num_experts, n, k); zeros for experts without rows.
+    """
+    _check_matrix(grad, 2)
+    _check_matrix(x, 2)
+    device = x.device
+    assert grad.device == device and grad.shape[0] == x.shape[0]
+    assert out_dtype in (torch.float32, torch.bfloat16)
+    num_rows, n, k = x.shape[0], grad.shape[1], x.shape[1]
+    num_experts = expert_start.numel()
+    assert num_experts >= 1
+    _check_groups(expert_start, expert_end, num_experts, device)
+    if out is None:
+        assert not accumulate, 'accumulate needs out'
+        out = torch.empty((num_experts, n, k), dtype=out_dtype, device=device)
+    else:
+        assert tuple(out.shape) == (num_experts, n, k) and out.dtype == out_dtype and out.device == device and out.is_contiguous()
+        assert not accumulate or out_dtype == torch.float32, 'accumulate needs a float32 destination'
+    if n > 0 and k > 0:
+        with device_guard(device):
+            rc = _lib.lib().tkq_grouped_gemm_wgrad(grad.data_ptr(), grad.stride(0), x.data_ptr(), x.stride(0), expert_start.data_ptr(),
+                                                   expert_end.data_ptr(), num_experts, num_rows, n, k, DTYPE_TO_ENUM[out_dtype],
+                                                   out.data_ptr(), _lib.ACCUMULATE if accumulate else 0, current_stream_ptr(device))
+        _lib.check(rc, 'tkq_grouped_gemm_wgrad')
+    return out

@@ -6,6 +6,7 @@ import torch
 from .. import _lib
 from .cast_back_e5m6_kernel import cast_back_e5m6, launch_cast_back
 from .common import get_cast_input_and_config, get_logical_hidden
+from .per_token_cast_to_nvfp4_kernel import cast_back_nvfp4
 from .types import QuantTensor
 
 
@@ -14,6 +15,7 @@ def cast_back(
     fmt: str,
     x_block_size: tuple[int, int],
     x_special_fmt: Optional[str] = None,
+    tensor_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Dequantise an FP8 / FP4 (or, with x_special_fmt='e5m6', packed E5M6) tensor to bfloat16 or float32.
 
@@ -21,9 +23,15 @@ def cast_back(
         x: (data, scales); data float8_e4m3fn or int8 (two FP4 per byte); scales in any layout the casts produce.
         fmt: 'bf16' or 'fp32'.
         x_block_size: scale block (tokens, channels).
+        tensor_scale: the scale per tensor of FP4 data with float8_e4m3fn scales (per_token_cast_to_nvfp4), whose
+            x_block_size is (1, 16); None for every other format.
     """
     assert fmt in ('bf16', 'fp32')
     data, x_sf = x
+    if x_sf.dtype == torch.float8_e4m3fn:
+        assert x_special_fmt is None and tuple(x_block_size) == (1, 16)
+        return cast_back_nvfp4((data, x_sf), fmt, tensor_scale)
+    assert tensor_scale is None, 'only float8_e4m3fn scales come with a scale per tensor'
     if x_special_fmt == 'e5m6':
         assert data.dtype == torch.uint8
         return cast_back_e5m6((data, x_sf), fmt, x_block_size)
