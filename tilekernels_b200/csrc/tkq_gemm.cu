@@ -25,15 +25,16 @@ struct Operand {
     bool bf16;
 };
 
-static int encode(CUtensorMap* map, const Operand& o, uint32_t box_inner, uint32_t box_rows) {
+static int encode(CUtensorMap* map, const Operand& o, uint32_t box_inner, uint32_t box_rows, bool fp32_out = false) {
     auto fn = tensor_map_encoder();
     if (fn == nullptr) return set_error(TKQ_E_UNSUPPORTED, "cuTensorMapEncodeTiled is not available from this driver");
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(o.inner), static_cast<cuuint64_t>(o.rows), static_cast<cuuint64_t>(o.groups)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.row_bytes), static_cast<cuuint64_t>(o.group_bytes)};
     const cuuint32_t box[3] = {box_inner, box_rows, 1};
     const cuuint32_t steps[3] = {1, 1, 1};
-    const CUresult r = fn(map, o.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(o.base), dims,
-                          strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const CUtensorMapDataType type = fp32_out ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : o.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const CUresult r = fn(map, type, 3, const_cast<void*>(o.base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          fp32_out ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(TKQ_E_UNSUPPORTED, "cuTensorMapEncodeTiled rejected an operand (alignment or size)");
     return 0;
@@ -49,19 +50,27 @@ static bool fix_strides(Operand& o) {
 
 template <class C>
 static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const char* what, cudaStream_t stream) {
-    alignas(64) CUtensorMap map_a, map_b;
+    alignas(64) CUtensorMap map_a, map_b, map_out{};
     if (int rc = encode(&map_a, a, C::A_MN ? 64 : C::kElems, C::A_MN ? 64 : 128)) return rc;
     if (int rc = encode(&map_b, b, C::WGRAD ? 64 : C::kElems, C::WGRAD ? 64 : C::kBRows)) return rc;
+    if (C::WGRAD && p.out_f32) {
+        const Operand o{p.out, p.i_size, p.j_size, p.groups, p.out_stride * 4, p.out_group_stride * 4, false};
+        p.wide_out = o.row_bytes % 16 == 0 && aligned16(o.base);
+        if (p.wide_out)
+            if (int rc = encode(&map_out, o, 32, 16, true)) return rc;
+    } else {
+        p.wide_out = p.i_size % 8 == 0 && p.out_stride % 8 == 0 && p.out_group_stride % 8 == 0 && aligned16(p.out);
+    }
     p.i_tiles = (p.i_size + 128 * C::CG - 1) / (128 * C::CG);
     const int64_t j_tiles = C::WGRAD ? int64_t{p.groups} * ((p.j_size + C::NMAX - 1) / C::NMAX) : int64_t{p.rows} / C::NMAX + p.groups;
     if (j_tiles * p.i_tiles >= (int64_t{1} << 31)) return set_error(TKQ_E_UNSUPPORTED, "matrix product: more than 2^31 tiles");
     const int64_t units = std::min<int64_t>(j_tiles * p.i_tiles, device_sm_count() / C::CG);
-    const int smem = static_cast<int>(1024 + C::kStages * C::kStageBytes + 4 * (3 * p.groups + 1));
+    const int smem = static_cast<int>(1024 + C::kStages * C::kStageBytes + C::kStagingBytes + 4 * (3 * p.groups + 1));
     auto kernel = gemm_kernel<C>;
     if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(units * C::CG));
-    config.blockDim = dim3(kGemmThreads);
+    config.blockDim = dim3(C::kThreads);
     config.dynamicSmemBytes = static_cast<size_t>(smem);
     config.stream = stream;
     cudaLaunchAttribute attr{};
@@ -70,7 +79,7 @@ static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const c
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = C::CG > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, map_a, map_b, p);
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, map_a, map_b, map_out, p);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return set_error(static_cast<int>(e), cudaGetErrorString(e));
@@ -79,11 +88,11 @@ static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const c
 }
 
 // Tile variant by the mean number of rows per group.
-template <int KIND, int NLARGE, bool A_MN>
+template <int KIND, int NMID, int NLARGE, bool A_MN>
 static int launch_rows(const Operand& a, const Operand& b, const GemmParams& p, const char* what, cudaStream_t stream) {
     const int64_t mean = p.rows / p.groups;
     if (mean <= 32) return launch_gemm<GemmConfig<KIND, 1, 32, false, A_MN>>(a, b, p, what, stream);
-    if (mean <= 128) return launch_gemm<GemmConfig<KIND, 1, 128, false, A_MN>>(a, b, p, what, stream);
+    if (mean <= 128) return launch_gemm<GemmConfig<KIND, 1, NMID, false, A_MN>>(a, b, p, what, stream);
     return launch_gemm<GemmConfig<KIND, 2, NLARGE, false, A_MN>>(a, b, p, what, stream);
 }
 
@@ -141,10 +150,9 @@ extern "C" int tkq_block_scaled_gemm(const void* x, int64_t x_row_stride, const 
     p.rows = static_cast<uint32_t>(num_rows);
     p.i_size = static_cast<uint32_t>(n);
     const int64_t row_bytes = k / per_byte;
-    p.k_blocks = static_cast<uint32_t>((row_bytes + 127) / 128);
-    p.last_units = static_cast<uint32_t>((row_bytes - (int64_t{p.k_blocks} - 1) * 128) / 32);
+    p.k_stages = static_cast<uint32_t>((row_bytes + 255) / 256);
+    p.last_units = static_cast<uint32_t>((row_bytes - (int64_t{p.k_stages} - 1) * 256) / 32);
     p.zero_gaps = (flags & TKQ_ZERO_GAPS) ? 1 : 0;
-    p.pair_stores = n % 2 == 0 && out_row_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
     auto view = [&](const void* sf, int64_t e, int64_t r, int64_t q, int shift, int block_k) {
         ScaleView v{};
         v.base = static_cast<const uint32_t*>(sf);
@@ -154,15 +162,15 @@ extern "C" int tkq_block_scaled_gemm(const void* x, int64_t x_row_stride, const 
         v.row_shift = static_cast<uint32_t>(shift);
         v.words = static_cast<uint32_t>((k + 4 * block_k - 1) / (4 * block_k));
         v.k_shift = block_k == 128 ? 2 : 0;
-        v.vec = q == 1 && r % 4 == 0 && e % 4 == 0 && aligned16(sf);
+        v.vec = q == 1 && r % 8 == 0 && e % 8 == 0 && reinterpret_cast<uintptr_t>(sf) % 32 == 0;
         return v;
     };
     p.sfa = view(w_sf, w_sf_expert_stride, w_sf_row_stride, w_sf_k_stride, ws, w_block_k);
     p.sfb = view(x_sf, 0, x_sf_row_stride, x_sf_k_stride, xs, x_block_k);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (fp8) return launch_rows<kKindMxf8, 224, false>(a, b, p, "block_scaled_gemm", s);
-    if (!nv) return launch_rows<kKindMxf4, 224, false>(a, b, p, "block_scaled_gemm", s);
-    return launch_rows<kKindNvf4, 192, false>(a, b, p, "block_scaled_gemm", s);
+    if (fp8) return launch_rows<kKindMxf8, 128, 224, false>(a, b, p, "block_scaled_gemm", s);
+    if (!nv) return launch_rows<kKindMxf4, 128, 224, false>(a, b, p, "block_scaled_gemm", s);
+    return launch_rows<kKindNvf4, 96, 192, false>(a, b, p, "block_scaled_gemm", s);
 }
 
 extern "C" int tkq_grouped_gemm(const void* x, int64_t x_row_stride, const void* w, int64_t w_expert_stride, int64_t w_row_stride, int transpose_w,
@@ -185,13 +193,12 @@ extern "C" int tkq_grouped_gemm(const void* x, int64_t x_row_stride, const void*
     p.groups = static_cast<uint32_t>(num_experts);
     p.rows = static_cast<uint32_t>(num_rows);
     p.i_size = static_cast<uint32_t>(n);
-    p.k_blocks = static_cast<uint32_t>((k + 63) / 64);
-    p.last_units = static_cast<uint32_t>((k - (int64_t{p.k_blocks} - 1) * 64 + 15) / 16);
+    p.k_stages = static_cast<uint32_t>((k + 63) / 64);
+    p.last_units = static_cast<uint32_t>((k - (int64_t{p.k_stages} - 1) * 64 + 15) / 16);
     p.zero_gaps = (flags & TKQ_ZERO_GAPS) ? 1 : 0;
-    p.pair_stores = n % 2 == 0 && out_row_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (transpose_w) return launch_rows<kKindBf16, 256, true>(a, b, p, "grouped_gemm", s);
-    return launch_rows<kKindBf16, 256, false>(a, b, p, "grouped_gemm", s);
+    if (transpose_w) return launch_rows<kKindBf16, 128, 256, true>(a, b, p, "grouped_gemm", s);
+    return launch_rows<kKindBf16, 128, 256, false>(a, b, p, "grouped_gemm", s);
 }
 
 extern "C" int tkq_grouped_gemm_wgrad(const void* grad, int64_t grad_row_stride, const void* x, int64_t x_row_stride, const int32_t* expert_start,
@@ -226,7 +233,6 @@ extern "C" int tkq_grouped_gemm_wgrad(const void* grad, int64_t grad_row_stride,
     p.j_size = static_cast<uint32_t>(n);
     p.out_f32 = out_dtype == TKQ_DT_FP32;
     p.accumulate = (flags & TKQ_ACCUMULATE) ? 1 : 0;
-    p.pair_stores = k % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true>>(a, b, p, "grouped_gemm_wgrad", s);
 }

@@ -20,12 +20,13 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "tkq_launch.cuh"
 #include "tkq_tcgen05.cuh"
 
 namespace tkq {
 
-constexpr int kGemmThreads = 256;
 constexpr int kMaxGroups = 1024;
 constexpr uint32_t kGemmSmemBudget = 232448 - 1024 /* alignment */ - 512 /* barriers */ - 12 * (kMaxGroups + 1);
 
@@ -37,7 +38,7 @@ struct ScaleView {
     uint32_t row_shift;
     uint32_t words;      // words along K
     uint32_t k_shift;    // 2: a byte covers 128 values (one word per four stages), 0: 32 or 16 values
-    uint32_t vec;        // the words of a row lie together on 16-byte boundaries
+    uint32_t vec;        // the words of a row lie together on 32-byte boundaries
 };
 
 struct GemmParams {
@@ -51,35 +52,45 @@ struct GemmParams {
     uint32_t groups, rows;     // rows: of the operand with the ragged axis
     uint32_t i_size, j_size;   // j_size: weight gradient only
     uint32_t i_tiles;
-    uint32_t k_blocks, last_units;  // forward: stages along K, matrix instructions of the last one
+    uint32_t k_stages, last_units;  // forward: stages along K, matrix instructions of the last one
     uint32_t alpha_stride;
-    uint32_t out_f32, accumulate, zero_gaps, pair_stores;
+    uint32_t out_f32, accumulate, zero_gaps;
+    uint32_t wide_out;  // bf16: rows of out on 16-byte boundaries and i_size a multiple of 8; fp32: map_out is set
 };
 
 template <int KIND_, int CG_, int NMAX_, bool WGRAD_, bool A_MN_>
 struct GemmConfig {
     static constexpr int KIND = KIND_, CG = CG_, NMAX = NMAX_;
     static constexpr bool WGRAD = WGRAD_, A_MN = A_MN_, SCALED = KIND_ != kKindBf16;
+    // A stage holds kSub blocks of 128 bytes along K.  Waiting for a stage and handing it back costs the issuing warp some
+    // 200 cycles: two thirds of a block's products in 4 or 8 bits (448 cycles at N = 224), which therefore come in pairs
+    static constexpr uint32_t kSub = SCALED ? 2 : 1;
     static constexpr uint32_t kBRows = NMAX / CG;
-    static constexpr uint32_t kABytes = 128 * 128, kBBytes = kBRows * 128;
+    static constexpr uint32_t kABytes = 128 * 128, kBBytes = kBRows * 128;  // of one block
     static constexpr uint32_t kWords = KIND == kKindMxf8 ? 1 : KIND == kKindMxf4 ? 2 : KIND == kKindNvf4 ? 4 : 0;
     static constexpr uint32_t kSfbBlocks = (NMAX + 127) / 128;
     static constexpr uint32_t kSfaBytes = 512 * kWords, kSfbBytes = 512 * kWords * kSfbBlocks;
-    static constexpr uint32_t kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
-    static constexpr uint32_t kStages = kGemmSmemBudget / kStageBytes < 12 ? kGemmSmemBudget / kStageBytes : 12;
-    static constexpr uint32_t kSfCols = 4 * kWords * (1 + kSfbBlocks);  // tensor-memory columns of one stage's scales
+    static constexpr uint32_t kStageBytes = kSub * (kABytes + kBBytes + kSfaBytes + kSfbBytes);
+    static constexpr uint32_t kLoaders = SCALED ? 6 : 2;  // warps between the two issuing ones and those that store results
+    static constexpr uint32_t kFirstResultWarp = 2 + kLoaders, kResultWarps = SCALED ? 4 : 8;
+    static constexpr uint32_t kThreads = 32 * (kFirstResultWarp + kResultWarps);
+    static constexpr uint32_t kStagingPerWarp = SCALED ? 2048 : 4096, kStagingBytes = kStagingPerWarp * kResultWarps;
+    static constexpr uint32_t kFits = (kGemmSmemBudget - kStagingBytes) / kStageBytes;
+    static constexpr uint32_t kStages = kFits < 10 ? kFits : 10;
+    static constexpr uint32_t kSfCols = 4 * kWords * (1 + kSfbBlocks);  // tensor-memory columns of one block's scales
     static constexpr uint32_t kSfBase = 2 * NMAX;
-    static constexpr uint32_t kColsNeeded = 2 * NMAX + 2 * kSfCols;
+    static constexpr uint32_t kColsNeeded = 2 * NMAX + kSub * kSfCols;
     static constexpr uint32_t kCols = kColsNeeded <= 64 ? 64 : kColsNeeded <= 128 ? 128 : kColsNeeded <= 256 ? 256 : 512;
     static constexpr uint32_t kElems = KIND == kKindBf16 ? 64 : 128;  // tensor-map elements of a 128-byte row
     static constexpr uint32_t kNStep = CG == 2 ? 32 : 16;
     static_assert(kColsNeeded <= 512, "tensor memory");
-    static_assert(!WGRAD || (A_MN && kBRows % 64 == 0), "weight gradient reads both operands along their rows");
-    static_assert(kBBytes % 1024 == 0 && kStages >= 4, "stage layout");
+    static_assert(kFirstResultWarp % 4 == 0, "a warp reads the quarter of tensor memory of its number modulo four");
+    static_assert(!WGRAD || (A_MN && kBRows % 64 == 0 && kSub == 1), "weight gradient reads both operands along their rows");
+    static_assert(kBBytes % 1024 == 0 && kStages >= 3, "stage layout");
 };
 
 struct GemmTile {
-    uint32_t e, i0, j0, jn, n_mma, k0, k_blocks, k_rows;
+    uint32_t e, i0, j0, jn, n_mma, k0, k_stages, k_rows;
 };
 
 __device__ unsigned int g_gemm_wait_failed = 0;
@@ -143,7 +154,7 @@ struct GemmSchedule {
         r.n_mma = (r.jn + C::kNStep - 1) / C::kNStep * C::kNStep;
         r.k0 = C::WGRAD ? start[r.e] : 0;
         r.k_rows = C::WGRAD ? rows[r.e] : 0;
-        r.k_blocks = C::WGRAD ? (rows[r.e] + 63) / 64 : p.k_blocks;
+        r.k_stages = C::WGRAD ? (rows[r.e] + 63) / 64 : p.k_stages;
         return r;
     }
 };
@@ -151,24 +162,30 @@ struct GemmSchedule {
 // Scale words of ROWBLK * 32 rows for one stage: lane l holds rows l, l + 32, ...
 template <class C, int ROWBLK>
 struct ScaleRegs {
-    uint32_t w[ROWBLK][C::kWords > 0 ? C::kWords : 1];
+    static constexpr uint32_t kStageWords = C::kSub * C::kWords;
+    uint32_t w[ROWBLK][kStageWords];
 
-    __device__ __forceinline__ void load(const ScaleView& v, const uint32_t* group, uint32_t row0, uint32_t row_end, uint32_t kb, uint32_t lane) {
-        const uint32_t word0 = C::KIND == kKindMxf8 ? kb >> v.k_shift : kb * C::kWords;
+    __device__ __forceinline__ void load(const ScaleView& v, const uint32_t* group, uint32_t row0, uint32_t row_end, uint32_t stage, uint32_t lane) {
+        const uint32_t word0 = v.k_shift ? stage >> 1 : stage * kStageWords;  // scales of 128 values: one word for two stages
 #pragma unroll
         for (int c = 0; c < ROWBLK; ++c) {
             const uint32_t row = row0 + lane + 32u * c;
             const uint32_t* at = group + static_cast<int64_t>(row >> v.row_shift) * v.row_stride + static_cast<int64_t>(word0) * v.k_stride;
             const bool valid = row < row_end;
-            if constexpr (C::kWords == 4) {
-                if (v.vec && word0 + 4 <= v.words) {
-                    uint4 q = valid ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
-                    w[c][0] = q.x, w[c][1] = q.y, w[c][2] = q.z, w[c][3] = q.w;
+            if constexpr (C::KIND == kKindNvf4) {
+                if (v.vec && word0 + kStageWords <= v.words) {  // the 32 bytes of a row in one load
+#pragma unroll
+                    for (uint32_t k = 0; k < kStageWords; ++k) w[c][k] = 0;
+                    if (valid)
+                        asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                                     : "=r"(w[c][0]), "=r"(w[c][1]), "=r"(w[c][2]), "=r"(w[c][3]), "=r"(w[c][4]), "=r"(w[c][5]), "=r"(w[c][6]), "=r"(w[c][7])
+                                     : "l"(at));
                     continue;
                 }
             }
 #pragma unroll
-            for (uint32_t k = 0; k < C::kWords; ++k) w[c][k] = valid && word0 + k < v.words ? __ldg(at + k * v.k_stride) : 0u;
+            for (uint32_t k = 0; k < kStageWords; ++k)
+                w[c][k] = valid && word0 + k < v.words && (k == 0 || !v.k_shift) ? __ldg(at + k * v.k_stride) : 0u;
         }
     }
 
@@ -176,7 +193,7 @@ struct ScaleRegs {
     __device__ __forceinline__ void store(uint32_t smem, uint32_t lane) const {
         constexpr int kBlocks = (ROWBLK + 3) / 4;
 #pragma unroll
-        for (uint32_t k = 0; k < C::kWords; ++k)
+        for (uint32_t k = 0; k < kStageWords; ++k)
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 uint32_t q[4];
@@ -189,9 +206,130 @@ struct ScaleRegs {
     }
 };
 
+// A scale loader's place: stage `stage` of tile `tile`, the block's stage number `it`.
 template <class C>
-__global__ void __launch_bounds__(kGemmThreads, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmParams p) {
+struct ScaleWalk {
+    GemmTile tile;
+    uint32_t t, stage, it;
+    bool valid;
+
+    __device__ __forceinline__ void begin(const GemmParams& p, const GemmSchedule<C>& sched, uint32_t unit) {
+        t = unit;
+        stage = it = 0;
+        valid = t < sched.total;
+        if (valid) tile = sched.tile(p, t);
+    }
+    __device__ __forceinline__ void advance(const GemmParams& p, const GemmSchedule<C>& sched, uint32_t units, uint32_t stages) {
+        stage += stages;
+        it += stages;
+        while (valid && stage >= p.k_stages) {
+            stage -= p.k_stages;
+            t += units;
+            valid = t < sched.total;
+            if (valid) tile = sched.tile(p, t);
+        }
+    }
+};
+
+// 32 columns of the accumulator (rows j of the output) of a warp's 32 lanes (its columns i) -> bf16.  The fragments of a
+// 16-lane load are those of an 8 x 8 matrix store, which transposes them on the way into shared memory (64-byte rows, 16-byte
+// chunks permuted so that neither side meets a bank twice); from there every lane moves 16 bytes of a row at a time.
+template <class C>
+__device__ __forceinline__ void store_bf16(const GemmParams& p, const GemmTile& tile, uint32_t (&v)[32], bool have, uint32_t taddr, uint32_t iw,
+                                           uint32_t c, uint32_t n, float alpha, uint32_t smem, uint32_t lane) {
+    if (have) {
+        tmem_load_16x32(taddr, v);
+        tmem_load_16x32(taddr + (16u << 16), v + 16);
+        tmem_load_wait();
+    } else {
+#pragma unroll
+        for (int q = 0; q < 32; ++q) v[q] = 0;
+    }
+#pragma unroll
+    for (uint32_t half = 0; half < 2; ++half)
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            uint32_t m[4];
+#pragma unroll
+            for (uint32_t x = 0; x < 4; ++x) {
+                const float lo = __uint_as_float(v[16 * half + 4 * x + 2 * h]), hi = __uint_as_float(v[16 * half + 4 * x + 2 * h + 1]);
+                const __nv_bfloat162 b = __floats2bfloat162_rn(__fmul_rn(lo, alpha), __fmul_rn(hi, alpha));
+                m[x] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            const uint32_t chunk = (half * 2 + h) ^ ((lane >> 1) & 3u);
+            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem + lane * 64u + chunk * 16u), "r"(m[0]),
+                         "r"(m[1]), "r"(m[2]), "r"(m[3])
+                         : "memory");
+        }
+    __syncwarp();
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + static_cast<int64_t>(tile.e) * p.out_group_stride +
+                         static_cast<int64_t>(tile.j0 + c) * p.out_stride + iw;
+    if (p.wide_out) {
+        const uint32_t chunk = lane & 3u;
+        const bool in = iw + chunk * 8 < p.i_size;
+        __nv_bfloat16* o = out + static_cast<int64_t>(lane >> 2) * p.out_stride + chunk * 8;
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q) {
+            const uint32_t row = q * 8 + (lane >> 2);
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(smem + row * 64u + ((chunk ^ ((row >> 1) & 3u)) * 16u)));
+            if (in && row < n) *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+            o += 8 * p.out_stride;
+        }
+    } else if (iw + lane < p.i_size) {
+        for (uint32_t row = 0; row < n; ++row) {
+            uint16_t w;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(smem + row * 64u + (((lane >> 3) ^ ((row >> 1) & 3u)) * 16u) + (lane & 7u) * 2u));
+            reinterpret_cast<uint16_t*>(out + static_cast<int64_t>(row) * p.out_stride)[lane] = w;
+        }
+    }
+}
+
+// The same for fp32 results of the weight gradient: rows of 128 bytes in shared memory leave by TMA, 16 rows at a time,
+// cut off at the tensor's edges; an accumulating call has them added in L2 (each element once).
+template <class C>
+__device__ __forceinline__ void store_f32(const GemmParams& p, const CUtensorMap& map_out, const GemmTile& tile, uint32_t (&v)[32], bool have,
+                                          uint32_t taddr, uint32_t iw, uint32_t c, uint32_t n, uint32_t smem, uint32_t& turn, uint32_t lane) {
+    if (have) {
+        tmem_load32(taddr, v);
+        tmem_load_wait();
+    } else {
+#pragma unroll
+        for (int q = 0; q < 32; ++q) v[q] = 0;
+    }
+    if (p.wide_out) {
+#pragma unroll
+        for (uint32_t half = 0; half < 2; ++half) {
+            const uint32_t buf = smem + (turn & 1u) * 2048u;
+            if (lane == 0) bulk_store_wait_read<1>();  // the store before the last one has left this half
+            __syncwarp();
+#pragma unroll
+            for (uint32_t q = 0; q < 16; ++q) asm volatile("st.shared.b32 [%0], %1;" ::"r"(buf + q * 128u + lane * 4u), "r"(v[16 * half + q]) : "memory");
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && iw < p.i_size && 16 * half < n)
+                tma_store_3d(&map_out, buf, static_cast<int32_t>(iw), static_cast<int32_t>(tile.j0 + c + 16 * half), static_cast<int32_t>(tile.e),
+                             p.accumulate != 0);
+            if (lane == 0) bulk_store_commit();
+            ++turn;
+        }
+    } else if (iw + lane < p.i_size) {
+        float* o = static_cast<float*>(p.out) + static_cast<int64_t>(tile.e) * p.out_group_stride + static_cast<int64_t>(tile.j0 + c) * p.out_stride + iw + lane;
+#pragma unroll
+        for (uint32_t q = 0; q < 32; ++q)
+            if (q < n) {
+                float* at = o + static_cast<int64_t>(q) * p.out_stride;
+                *at = p.accumulate ? __fadd_rn(*at, __uint_as_float(v[q])) : __uint_as_float(v[q]);
+            }
+    }
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::kThreads, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out,
+                const GemmParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full_bar[C::kStages], empty_bar[C::kStages], ready_bar[C::kStages], acc_full[2], acc_empty[2], drain_bar;
     __shared__ uint32_t tmem_slot;
@@ -202,8 +340,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const uint32_t unit = blockIdx.x / C::CG, units = gridDim.x / C::CG;
 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t a_base = base, b_base = a_base + C::kStages * C::kABytes, sf_base = b_base + C::kStages * C::kBBytes;
-    uint32_t* group_mem = reinterpret_cast<uint32_t*>(smem_raw + (base - smem_u32(smem_raw)) + C::kStages * C::kStageBytes);
+    const uint32_t a_base = base, b_base = a_base + C::kStages * C::kSub * C::kABytes, staging = b_base + C::kStages * C::kSub * C::kBBytes;
+    const uint32_t sf_base = staging + C::kStagingBytes;
+    uint32_t* group_mem = reinterpret_cast<uint32_t*>(smem_raw + (base - smem_u32(smem_raw)) + C::kStages * C::kStageBytes + C::kStagingBytes);
     uint32_t* s_prefix = group_mem;
     uint32_t* s_start = s_prefix + p.groups + 1;
     uint32_t* s_rows = s_start + p.groups;
@@ -250,7 +389,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
             for (int a = 0; a < 2; ++a) {
                 mbar_init(&acc_full[a], 1);
-                mbar_init(&acc_empty[a], 4 * C::CG);
+                mbar_init(&acc_empty[a], C::kResultWarps * C::CG);
             }
             mbar_init(&drain_bar, 1);
         }
@@ -269,170 +408,194 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     auto bar = [](uint64_t* b) { return smem_u32(b); };
     auto leader_bar = [&](uint64_t* b) { return C::CG == 2 ? map_to_rank(smem_u32(b), 0) : smem_u32(b); };
 
+    // The two issuing warps run their loops whole, with one lane elected for the waits and the instructions: in a branch that
+    // a lane enters alone, every operand of every instruction is moved into uniform registers first.  Per stage of four
+    // bf16 products of 256 x 256 x 16 (512 cycles): 875 cycles with the loop in one lane's branch, 600 with a branch around the
+    // instructions, 518 with predicated instructions and one polling lane that looks at the next stage ahead of time.
     if (warp == 0) {
-        if (lane == 0) {
-            // ---- operand tiles ----
-            uint32_t it = 0;
-            bool ok = true;
-            for (uint32_t t = unit; ok && t < sched.total; t += units) {
-                const GemmTile tile = sched.tile(p, t);
-                const int32_t i0 = static_cast<int32_t>(tile.i0 + rank * 128u);
-                const int32_t j0 = static_cast<int32_t>(tile.j0 + (C::CG == 2 ? rank * (tile.n_mma / 2) : 0));
-                for (uint32_t kb = 0; kb < tile.k_blocks; ++kb, ++it) {
-                    const uint32_t s = it % C::kStages;
-                    if (!(ok = wait(bar(&empty_bar[s]), ((it / C::kStages) & 1u) ^ 1u))) break;
-                    uint32_t full;
-                    if constexpr (C::WGRAD) {
-                        full = bar(&full_bar[s]);
-                        mbar_arrive_expect_tx(&full_bar[s], C::kABytes + C::kBBytes);
-                    } else {
-                        full = leader_bar(&full_bar[s]);
-                        if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], C::CG * (C::kABytes + C::kBBytes));
-                    }
-                    const uint32_t a = a_base + s * C::kABytes, b = b_base + s * C::kBBytes;
-                    const int32_t k = static_cast<int32_t>(tile.k0 + kb * C::kElems);
-                    if constexpr (C::A_MN) {
-                        const int32_t z = C::WGRAD ? 0 : static_cast<int32_t>(tile.e);
-                        tma_load_3d<C::CG>(a, &map_a, i0, k, z, full);
-                        tma_load_3d<C::CG>(a + 8192, &map_a, i0 + 64, k, z, full);
-                    } else {
-                        tma_load_3d<C::CG>(a, &map_a, k, i0, static_cast<int32_t>(tile.e), full);
-                    }
-                    if constexpr (C::WGRAD) {
+        // ---- operand tiles ----
+        const bool one = elect_one();
+        uint32_t s = 0, phase = 1, filled = 0;
+        bool ok = true;
+        for (uint32_t t = unit; ok && t < sched.total; t += units) {
+            const GemmTile tile = sched.tile(p, t);
+            const int32_t i0 = static_cast<int32_t>(tile.i0 + rank * 128u);
+            const int32_t j0 = static_cast<int32_t>(tile.j0 + (C::CG == 2 ? rank * (tile.n_mma / 2) : 0));
+            const uint32_t k_stages = C::WGRAD ? tile.k_stages : p.k_stages;
+            for (uint32_t kb = 0; kb < k_stages; ++kb) {
+                ok = __any_sync(kFullMask, one && wait(bar(&empty_bar[s]), phase));
+                if (!ok) break;
+                const uint32_t a = a_base + s * (C::kSub * C::kABytes), b = b_base + s * (C::kSub * C::kBBytes);
+                const int32_t k = static_cast<int32_t>(tile.k0 + kb * (C::kSub * C::kElems));
+                const uint32_t full = C::WGRAD ? bar(&full_bar[s]) : leader_bar(&full_bar[s]);
+                if (one) {
+                    if (C::WGRAD) mbar_arrive_expect_tx(&full_bar[s], C::kABytes + C::kBBytes);
+                    else if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], C::CG * C::kSub * (C::kABytes + C::kBBytes));
 #pragma unroll
-                        for (uint32_t q = 0; q < C::kBRows / 64; ++q)
-                            tma_load_3d<C::CG>(b + q * 8192, &map_b, j0 + static_cast<int32_t>(64 * q), k, 0, full);
-                    } else {
-                        tma_load_3d<C::CG>(b, &map_b, k, j0, 0, full);
+                    for (uint32_t u = 0; u < C::kSub; ++u) {
+                        const int32_t ku = k + static_cast<int32_t>(u * C::kElems);
+                        if constexpr (C::A_MN) {
+                            const int32_t z = C::WGRAD ? 0 : static_cast<int32_t>(tile.e);
+                            tma_load_3d<C::CG>(a, &map_a, i0, ku, z, full);
+                            tma_load_3d<C::CG>(a + 8192, &map_a, i0 + 64, ku, z, full);
+                        } else {
+                            tma_load_3d<C::CG>(a + u * C::kABytes, &map_a, ku, i0, static_cast<int32_t>(tile.e), full);
+                        }
+                        if constexpr (C::WGRAD) {
+#pragma unroll
+                            for (uint32_t q = 0; q < C::kBRows / 64; ++q)
+                                tma_load_3d<C::CG>(b + q * 8192, &map_b, j0 + static_cast<int32_t>(64 * q), ku, 0, full);
+                        } else {
+                            tma_load_3d<C::CG>(b + u * C::kBBytes, &map_b, ku, j0, 0, full);
+                        }
                     }
                 }
-            }
-            // every stage that was filled has been read before the block may end
-            for (uint32_t n = 0; n < C::kStages && n < it; ++n) {
-                const uint32_t q = it - 1 - n;
-                if (ok) ok = wait(bar(&empty_bar[q % C::kStages]), (q / C::kStages) & 1u);
-                else if (C::WGRAD || rank == 0) mbar_wait(&full_bar[q % C::kStages], (q / C::kStages) & 1u, 1u << 16);
+                __syncwarp();
+                filled = min(filled + 1, C::kStages);
+                if (++s == C::kStages) s = 0, phase ^= 1;
             }
         }
+        // every stage that was filled has been read before the block may end
+        for (; filled > 0; --filled) {
+            const uint32_t back = filled;  // the stage filled `back` fills ago
+            const uint32_t q = s >= back ? s - back : s + C::kStages - back;
+            const uint32_t q_phase = s >= back ? phase ^ 1u : phase;  // parity of that fill's own phase
+            if (ok) ok = __any_sync(kFullMask, one && wait(bar(&empty_bar[q]), q_phase));
+            else if (C::WGRAD || rank == 0) mbar_wait(&full_bar[q], q_phase, 1u << 16);
+        }
     } else if (warp == 1) {
-        if (rank == 0 && lane == 0) {
+        if (rank == 0) {
             // ---- matrix instructions ----
             constexpr uint32_t kM = 128 * C::CG;
-            uint32_t it = 0, acc_it = 0;
-            bool ok = true;
+            // a step along K: 32 bytes of a K-major row, or 16 rows of 128 bytes
+            constexpr uint32_t kStepA = (C::A_MN ? 2048 : 32) >> 4, kStepB = (C::WGRAD ? 2048 : 32) >> 4;
+            const uint64_t desc_a = smem_desc(a_base, C::A_MN ? 8192 : 16, 1024, kSwizzle128);
+            const uint64_t desc_b = smem_desc(b_base, C::WGRAD ? 8192 : 16, 1024, kSwizzle128);
+            const uint64_t desc_sf = smem_desc(sf_base, 16, 128, 0);
+            // scale bytes of successive instructions: the next one (32 values each) or the same one (128 values)
+            const uint32_t id_step = idesc_scale_ids(p.sfa.k_shift ? 0 : 1, p.sfb.k_shift ? 0 : 1);
+            const uint32_t id_block = idesc_scale_ids(p.sfa.k_shift ? 1 : 0, p.sfb.k_shift ? 1 : 0);
+            const bool one = elect_one();
+            uint32_t s = 0, phase = 0, acc_it = 0;
+            bool ok = true, ready = false;  // ready: the next stage's operands have been seen to be there
             for (uint32_t t = unit; ok && t < sched.total; t += units) {
                 const GemmTile tile = sched.tile(p, t);
-                if (tile.k_blocks == 0) continue;
+                const uint32_t k_stages = C::WGRAD ? tile.k_stages : p.k_stages;
+                if (k_stages == 0) continue;
                 const uint32_t a = acc_it & 1u;
-                if (!(ok = wait(bar(&acc_empty[a]), ((acc_it >> 1) & 1u) ^ 1u))) break;
+                ok = __any_sync(kFullMask, one && wait(bar(&acc_empty[a]), ((acc_it >> 1) & 1u) ^ 1u));
+                if (!ok) break;
                 ++acc_it;
                 tcgen05_fence_after();
                 const uint32_t d = tmem + a * C::NMAX;
                 uint32_t idesc;
                 if constexpr (C::SCALED) idesc = idesc_scaled(kM, tile.n_mma, C::KIND == kKindMxf8 ? 0 : 1, C::KIND != kKindNvf4);
                 else idesc = idesc_bf16(kM, tile.n_mma, C::A_MN, C::WGRAD);
-                for (uint32_t kb = 0; kb < tile.k_blocks; ++kb, ++it) {
-                    const uint32_t s = it % C::kStages, phase = (it / C::kStages) & 1u;
-                    if (!(ok = wait(bar(C::WGRAD ? &ready_bar[s] : &full_bar[s]), phase))) break;
+                for (uint32_t kb = 0; kb < k_stages; ++kb) {
+                    if (!ready) ok = __any_sync(kFullMask, one && wait(bar(C::WGRAD ? &ready_bar[s] : &full_bar[s]), phase));
+                    if (!ok) break;
                     tcgen05_fence_after();
-                    const uint32_t sfa = tmem + C::kSfBase + (it & 1u) * C::kSfCols, sfb = sfa + 4 * C::kWords;
-                    if constexpr (C::SCALED) {
-                        // the copies overwrite the scales of two stages ago: its products have to be finished
-                        if (it >= 2) {
-                            const uint32_t q = it - 2;
-                            if (!(ok = wait(bar(&empty_bar[q % C::kStages]), (q / C::kStages) & 1u))) break;
-                            tcgen05_fence_after();
+                    const uint32_t now = s;
+                    if (++s == C::kStages) s = 0, phase ^= 1;
+                    bool seen = false;
+                    if (one) seen = mbar_try_wait_cluster(bar(C::WGRAD ? &ready_bar[s] : &full_bar[s]), phase);
+                    uint32_t n_units = 4 * C::kSub;
+                    if (kb + 1 == k_stages) n_units = C::WGRAD ? (tile.k_rows - kb * 64 + 15) / 16 : p.last_units;
+#pragma unroll
+                    for (uint32_t h = 0; h < C::kSub; ++h) {
+                        if (h > 0 && 4 * h >= n_units) break;
+                        const uint64_t da = desc_a + (now * C::kSub + h) * (C::kABytes >> 4), db = desc_b + (now * C::kSub + h) * (C::kBBytes >> 4);
+                        const uint32_t sfa = tmem + C::kSfBase + h * C::kSfCols, sfb = sfa + 4 * C::kWords;
+                        uint32_t id0 = idesc;
+                        if constexpr (C::SCALED) {
+                            // The copies go over the scales of the block two before.  Copies and products of one thread run in the
+                            // order of their issue (they share a pipe), so nothing has to be waited for.
+                            const uint64_t dfa = desc_sf + now * ((C::kSub * (C::kSfaBytes + C::kSfbBytes)) >> 4);
+                            const uint64_t dfb = dfa + ((C::kSub * C::kSfaBytes) >> 4);
+                            const uint32_t ha = C::KIND == kKindMxf8 && p.sfa.k_shift ? 0 : h, hb = C::KIND == kKindMxf8 && p.sfb.k_shift ? 0 : h;
+#pragma unroll
+                            for (uint32_t w = 0; w < C::kWords; ++w) {
+                                tcgen05_copy_scales<C::CG>(one, sfa + 4 * w, dfa + 32 * (ha * C::kWords + w));
+#pragma unroll
+                                for (uint32_t b = 0; b < C::kSfbBlocks; ++b)
+                                    tcgen05_copy_scales<C::CG>(one, sfb + 4 * (w * C::kSfbBlocks + b), dfb + 32 * ((hb * C::kWords + w) * C::kSfbBlocks + b));
+                            }
+                            if constexpr (C::KIND == kKindMxf8) id0 += id_block * ((kb & 1u) * 2 + h);
                         }
-                        const uint32_t sf = sf_base + s * (C::kSfaBytes + C::kSfbBytes);
 #pragma unroll
-                        for (uint32_t w = 0; w < C::kWords; ++w) {
-                            tcgen05_copy_scales<C::CG>(sfa + 4 * w, smem_desc(sf + 512 * w, 16, 128, 0));
-#pragma unroll
-                            for (uint32_t b = 0; b < C::kSfbBlocks; ++b)
-                                tcgen05_copy_scales<C::CG>(sfb + 4 * (w * C::kSfbBlocks + b),
-                                                           smem_desc(sf + C::kSfaBytes + 512 * (w * C::kSfbBlocks + b), 16, 128, 0));
+                        for (uint32_t u = 0; u < 4; ++u) {
+                            if (u > 0 && 4 * h + u >= n_units) break;
+                            uint32_t id = id0, fa = sfa, fb = sfb;
+                            if constexpr (C::KIND == kKindMxf8) id += u * id_step;
+                            if constexpr (C::KIND == kKindMxf4) {
+                                id |= idesc_scale_ids((u & 1u) * 2, (u & 1u) * 2);
+                                fa += 4 * (u >> 1);
+                                fb += 4 * C::kSfbBlocks * (u >> 1);
+                            }
+                            if constexpr (C::KIND == kKindNvf4) {
+                                fa += 4 * u;
+                                fb += 4 * C::kSfbBlocks * u;
+                            }
+                            tcgen05_mma<C::KIND, C::CG>(one, d, da + u * kStepA, db + u * kStepB, id, fa, fb, kb > 0 || h > 0 || u > 0);
                         }
                     }
-                    const uint32_t sa = a_base + s * C::kABytes, sb = b_base + s * C::kBBytes;
-                    uint64_t da, db;
-                    if constexpr (C::A_MN) da = smem_desc(sa, 8192, 1024, kSwizzle128);
-                    else da = smem_desc(sa, 16, 1024, kSwizzle128);
-                    if constexpr (C::WGRAD) db = smem_desc(sb, 8192, 1024, kSwizzle128);
-                    else db = smem_desc(sb, 16, 1024, kSwizzle128);
-                    // a step along K: 32 bytes of a K-major row, or 16 rows of 128 bytes
-                    constexpr uint32_t kStepA = (C::A_MN ? 2048 : 32) >> 4, kStepB = (C::WGRAD ? 2048 : 32) >> 4;
-                    uint32_t n_units = 4;
-                    if (kb + 1 == tile.k_blocks) n_units = C::WGRAD ? (tile.k_rows - kb * 64 + 15) / 16 : p.last_units;
-#pragma unroll
-                    for (uint32_t u = 0; u < 4; ++u) {
-                        if (u >= n_units) break;
-                        uint32_t id = idesc, fa = sfa, fb = sfb;
-                        if constexpr (C::KIND == kKindMxf8)
-                            id |= idesc_scale_ids(p.sfa.k_shift ? kb & 3u : u, p.sfb.k_shift ? kb & 3u : u);
-                        if constexpr (C::KIND == kKindMxf4) {
-                            id |= idesc_scale_ids((u & 1u) * 2, (u & 1u) * 2);
-                            fa += 4 * (u >> 1);
-                            fb += 4 * C::kSfbBlocks * (u >> 1);
-                        }
-                        if constexpr (C::KIND == kKindNvf4) {
-                            fa += 4 * u;
-                            fb += 4 * C::kSfbBlocks * u;
-                        }
-                        tcgen05_mma<C::KIND, C::CG>(d, da + u * kStepA, db + u * kStepB, id, fa, fb, kb > 0 || u > 0);
-                    }
-                    tcgen05_commit<C::CG>(bar(&empty_bar[s]));
+                    tcgen05_commit<C::CG>(one, bar(&empty_bar[now]));
+                    if (kb + 1 == k_stages) tcgen05_commit<C::CG>(one, bar(&acc_full[a]));
+                    ready = __any_sync(kFullMask, seen);
                 }
-                if (ok) tcgen05_commit<C::CG>(bar(&acc_full[a]));
             }
             if (!ok) {  // products in flight end before the memory they use is given up
-                tcgen05_commit<C::CG>(bar(&drain_bar));
+                tcgen05_commit<C::CG>(one, bar(&drain_bar));
                 mbar_wait(&drain_bar, 0, 1u << 16);
             }
         }
-    } else if (warp < 4) {
+    } else if (warp < C::kFirstResultWarp) {
         if constexpr (C::SCALED) {
-            // ---- scale factors: warp 2 those of A, warp 3 those of B; two stages of loads ahead of the stores ----
+            // ---- scale factors: even warps those of A, odd ones those of B.  Three warps per operand take stages in turn, each with
+            // the loads of its next stage in flight: the words come from L2 while TMA loads keep its ports busy, and take about
+            // a microsecond.  (8192 x 4096 x 7168 MXFP4 136 us with one warp per operand and loads two blocks ahead, 105 us
+            // without any loads.) ----
             auto run = [&](auto regs_tag, const ScaleView& v, uint32_t smem_off, bool is_a) {
                 using Regs = decltype(regs_tag);
-                uint32_t it = 0;
-                bool ok = true;
-                for (uint32_t t = unit; ok && t < sched.total; t += units) {
-                    const GemmTile tile = sched.tile(p, t);
-                    const uint32_t* group = v.base + (is_a ? static_cast<int64_t>(tile.e) * v.group_stride : 0);
-                    const uint32_t row0 = is_a ? tile.i0 + rank * 128u : tile.j0, row_end = is_a ? p.i_size : tile.j0 + tile.jn;
-                    Regs r[3];
-                    r[0].load(v, group, row0, row_end, 0, lane);
-                    if (tile.k_blocks > 1) r[1].load(v, group, row0, row_end, 1, lane);
-                    for (uint32_t kb = 0; kb < tile.k_blocks; kb += 3) {
+                Regs r[2];
+                ScaleWalk<C> at;
+                at.begin(p, sched, unit);
+                at.advance(p, sched, units, (warp - 2) >> 1);
+                auto load = [&](Regs& regs) {
+                    const GemmTile& tile = at.tile;
+                    regs.load(v, v.base + (is_a ? static_cast<int64_t>(tile.e) * v.group_stride : 0), is_a ? tile.i0 + rank * 128u : tile.j0,
+                              is_a ? p.i_size : tile.j0 + tile.jn, at.stage, lane);
+                };
+                if (at.valid) load(r[0]);
+                while (at.valid) {
 #pragma unroll
-                        for (uint32_t u = 0; u < 3; ++u) {
-                            if (kb + u >= tile.k_blocks) break;
-                            if (kb + u + 2 < tile.k_blocks) r[(u + 2) % 3].load(v, group, row0, row_end, kb + u + 2, lane);
-                            const uint32_t s = it % C::kStages;
-                            ok = wait(bar(&empty_bar[s]), ((it / C::kStages) & 1u) ^ 1u);
-                            if (!__all_sync(kFullMask, ok)) return;
-                            r[u].store(sf_base + s * (C::kSfaBytes + C::kSfbBytes) + smem_off, lane);
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive_cluster(C::CG == 2 ? map_to_rank(bar(&full_bar[s]), 0) : bar(&full_bar[s]));
-                            ++it;
-                        }
+                    for (int h = 0; h < 2; ++h) {
+                        if (!at.valid) break;
+                        const uint32_t it = at.it, s = it % C::kStages;
+                        at.advance(p, sched, units, C::kLoaders / 2);
+                        if (at.valid) load(r[h ^ 1]);
+                        const bool ok = wait(bar(&empty_bar[s]), ((it / C::kStages) & 1u) ^ 1u);
+                        if (!__all_sync(kFullMask, ok)) return;
+                        r[h].store(sf_base + s * (C::kSub * (C::kSfaBytes + C::kSfbBytes)) + smem_off, lane);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(leader_bar(&full_bar[s]));
                     }
                 }
             };
-            if (warp == 2) run(ScaleRegs<C, 4>{}, p.sfa, 0, true);
-            else run(ScaleRegs<C, (C::NMAX + 31) / 32>{}, p.sfb, C::kSfaBytes, false);
+            if ((warp & 1u) == 0) run(ScaleRegs<C, 4>{}, p.sfa, 0, true);
+            else run(ScaleRegs<C, (C::NMAX + 31) / 32>{}, p.sfb, C::kSub * C::kSfaBytes, false);
         } else if constexpr (C::WGRAD) {
             // ---- rows behind the group's end: the last stage's tail belongs to another group (or to nobody) and is cleared in
             // both operands, so that not even an infinity there can reach the sum ----
             if (warp == 2) {
-                uint32_t it = 0;
-                for (uint32_t t = unit; t < sched.total; t += units) {
+                uint32_t s = 0, phase = 0;
+                bool ok = true;
+                for (uint32_t t = unit; ok && t < sched.total; t += units) {
                     const GemmTile tile = sched.tile(p, t);
-                    for (uint32_t kb = 0; kb < tile.k_blocks; ++kb, ++it) {
-                        const uint32_t s = it % C::kStages;
-                        const bool ok = wait(bar(&full_bar[s]), (it / C::kStages) & 1u);
-                        if (!__all_sync(kFullMask, ok)) goto done;
+                    for (uint32_t kb = 0; kb < tile.k_stages; ++kb) {
+                        ok = __any_sync(kFullMask, lane == 0 && wait(bar(&full_bar[s]), phase));
+                        if (!ok) break;
                         const uint32_t valid = min(64u, tile.k_rows - kb * 64), padded = (valid + 15) / 16 * 16;
                         if (valid < padded) {
                             const uint32_t chunks = (padded - valid) * 8;
@@ -444,20 +607,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                             fence_proxy_async_smem();
                         }
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(C::CG == 2 ? map_to_rank(bar(&ready_bar[s]), 0) : bar(&ready_bar[s]));
+                        if (lane == 0) mbar_arrive_cluster(leader_bar(&ready_bar[s]));
+                        if (++s == C::kStages) s = 0, phase ^= 1;
                     }
                 }
-            done:;
             }
         }
     } else {
         // ---- results ----
-        const uint32_t quarter = warp & 3u;
-        uint32_t acc_it = 0;
+        const uint32_t quarter = warp & 3u, rw = warp - C::kFirstResultWarp;
+        const uint32_t stage_mem = staging + rw * C::kStagingPerWarp;
+        uint32_t acc_it = 0, turn = 0;
         for (uint32_t t = unit; t < sched.total; t += units) {
             const GemmTile tile = sched.tile(p, t);
             const uint32_t a = acc_it & 1u;
-            const bool have = tile.k_blocks > 0;
+            const bool have = tile.k_stages > 0;
             if (!have && p.accumulate) continue;
             if (have) {
                 const bool ok = wait(bar(&acc_full[a]), (acc_it >> 1) & 1u);
@@ -468,59 +632,28 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const float alpha = p.alpha == nullptr ? 1.0f : __ldg(p.alpha + static_cast<int64_t>(tile.e) * p.alpha_stride);
             const uint32_t iw = tile.i0 + rank * 128u + quarter * 32u;  // the warp's first column of the output
             const uint32_t taddr = tmem + a * C::NMAX + (quarter << 21);
-            for (uint32_t c = 0; c < tile.jn; c += 32) {
-                uint32_t v[32];
-                if (have) {
-                    tmem_load32(taddr + c, v);
-                    tmem_load_wait();
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 32; ++q) v[q] = 0;
-                }
-                const int64_t off = static_cast<int64_t>(tile.e) * p.out_group_stride + static_cast<int64_t>(tile.j0 + c) * p.out_stride;
+            for (uint32_t c = rw / 4 * 32; c < tile.jn; c += 8 * C::kResultWarps) {
                 const uint32_t n = min(32u, tile.jn - c);
+                uint32_t v[32];
                 if (C::WGRAD && p.out_f32) {
-                    float* o = static_cast<float*>(p.out) + off + iw + lane;
-                    if (iw + lane < p.i_size) {
-#pragma unroll
-                        for (uint32_t q = 0; q < 32; ++q)
-                            if (q < n) {
-                                float x = __uint_as_float(v[q]);
-                                if (p.accumulate) x += o[q * p.out_stride];
-                                o[q * p.out_stride] = x;
-                            }
-                    }
+                    store_f32<C>(p, map_out, tile, v, have, taddr + c, iw, c, n, stage_mem, turn, lane);
                 } else {
-                    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + off;
-                    if (p.pair_stores) {
-                        // two rows per step: lanes 0..15 store pairs of columns of row q, lanes 16..31 of row q + 1
-                        const uint32_t col = iw + 2 * (lane & 15u), src = 2 * (lane & 15u), upper = lane >> 4;
-#pragma unroll
-                        for (uint32_t q = 0; q < 32; q += 2) {
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(__fmul_rn(__uint_as_float(v[q]), alpha), __fmul_rn(__uint_as_float(v[q + 1]), alpha));
-                            const uint32_t mine = *reinterpret_cast<const uint32_t*>(&h);
-                            const uint32_t x = __shfl_sync(kFullMask, mine, src), y = __shfl_sync(kFullMask, mine, src + 1);
-                            const uint32_t w = __byte_perm(x, y, upper ? 0x7632 : 0x5410);
-                            if (q + upper < n && col < p.i_size) *reinterpret_cast<uint32_t*>(o + (q + upper) * p.out_stride + col) = w;
-                        }
-                    } else if (iw + lane < p.i_size) {
-#pragma unroll
-                        for (uint32_t q = 0; q < 32; ++q)
-                            if (q < n) o[q * p.out_stride + iw + lane] = __float2bfloat16_rn(__fmul_rn(__uint_as_float(v[q]), alpha));
-                    }
+                    store_bf16<C>(p, tile, v, have, taddr + c, iw, c, n, alpha, stage_mem + (turn & 1u) * 2048u, lane);
+                    if (C::kStagingPerWarp > 2048) ++turn;
+                    else __syncwarp();
                 }
             }
             if (have) {
                 tcgen05_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(C::CG == 2 ? map_to_rank(bar(&acc_empty[a]), 0) : bar(&acc_empty[a]));
+                if (lane == 0) mbar_arrive_cluster(leader_bar(&acc_empty[a]));
             }
         }
+        if (C::WGRAD && lane == 0) bulk_store_wait_all();
         if (!C::WGRAD && p.zero_gaps) {
             // rows of no group: before the first, between two, behind the last
-            const uint32_t w0 = blockIdx.x * 4 + quarter, nw = gridDim.x * 4;
-            const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && (p.out_stride & 7) == 0;
-            const uint32_t full8 = wide ? p.i_size / 8 : 0;
+            const uint32_t w0 = blockIdx.x * C::kResultWarps + rw, nw = gridDim.x * C::kResultWarps;
+            const uint32_t full8 = p.wide_out ? p.i_size / 8 : 0;
             for (uint32_t g = 0; g <= p.groups; ++g) {
                 const uint32_t lo = g == 0 ? 0 : s_start[g - 1] + s_rows[g - 1], hi = g == p.groups ? p.rows : s_start[g];
                 for (uint32_t r = lo + w0; r < hi; r += nw) {

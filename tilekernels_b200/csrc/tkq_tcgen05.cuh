@@ -30,14 +30,16 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
-// Arrival at a barrier of any CTA of the cluster (address from map_to_rank), releasing this thread's writes to it.
+// Arrival at a barrier of any CTA of the cluster (address from map_to_rank).  What it announces is shared or tensor memory
+// of the arriving thread's own SM, ordered by a proxy or tcgen05 fence before it.  With .release.cluster the same arrival
+// waits for the thread's global loads and costs about a microsecond (16384 x 4096 x 7168 MXFP4: 511 us with it, 377 us without).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t addr, uint32_t parity) {
     uint32_t done;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
                  : "=r"(done)
                  : "r"(addr), "r"(parity)
                  : "memory");
@@ -64,6 +66,21 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
             "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
             : "memory");
 }
+
+// Tile store (or addition, in L2) of a box in shared memory; what lies outside the tensor is left out.  Coordinates are not
+// negative, x * element size a multiple of 16 bytes.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* tmap, uint32_t smem_src, int32_t x, int32_t y, int32_t z, bool add) {
+    if (add)
+        asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tmap), "r"(x), "r"(y),
+                     "r"(z), "r"(smem_src)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tmap), "r"(x), "r"(y), "r"(z),
+                     "r"(smem_src)
+                     : "memory");
+}
+
+__device__ __forceinline__ void bulk_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
 // Tensor memory
@@ -97,6 +114,16 @@ __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
           "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
           "=r"(r[31])
+        : "r"(taddr));
+}
+
+// 16 lanes x 32 columns as 8 x 8 matrices: registers 4x and 4x + 1 of lane l are columns 8x + 2 (l % 4) and the next of
+// lane l / 4, registers 4x + 2 and 4x + 3 those of lane 8 + l / 4.
+__device__ __forceinline__ void tmem_load_16x32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
 
@@ -138,17 +165,21 @@ __device__ __forceinline__ uint32_t idesc_scale_ids(uint32_t a_id, uint32_t b_id
 // ---------------------------------------------------------------------------
 constexpr int kKindBf16 = 0, kKindMxf8 = 1, kKindMxf4 = 2, kKindNvf4 = 3;
 
+// The issuing functions are called by whole warps, with `one` true in a single lane: predicated instructions in
+// uniform control flow take their descriptors from uniform registers as they are, where a branch for one lane moves every
+// operand there first (about 60 cycles per instruction: 390 against 290 cycles for the four products of a bf16 stage).
 template <int KIND, int CG>
-__device__ __forceinline__ void tcgen05_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate) {
-    const uint32_t acc = accumulate ? 1u : 0u;
-#define TKQ_MMA_PLAIN(CGS, KINDS)                                                                                             \
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::" CGS ".kind::" KINDS " [%0], %1, %2, %3, p; }" ::"r"(d), \
-                 "l"(a), "l"(b), "r"(idesc), "r"(acc)                                                                         \
+__device__ __forceinline__ void tcgen05_mma(bool one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate) {
+    const uint32_t acc = accumulate ? 1u : 0u, e = one ? 1u : 0u;
+#define TKQ_MMA_PLAIN(CGS, KINDS)                                                                                                     \
+    asm volatile("{ .reg .pred e, p; setp.ne.b32 p, %4, 0; setp.ne.b32 e, %5, 0; @e tcgen05.mma.cta_group::" CGS ".kind::" KINDS     \
+                 " [%0], %1, %2, %3, p; }" ::"r"(d),                                                                                  \
+                 "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(e)                                                                         \
                  : "memory")
-#define TKQ_MMA_SCALED(CGS, KINDS)                                                                                                 \
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %6, 0; tcgen05.mma.cta_group::" CGS ".kind::" KINDS " [%0], %1, %2, %3, [%4], [%5], p; }" ::"r"( \
-                     d),                                                                                                           \
-                 "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)                                                          \
+#define TKQ_MMA_SCALED(CGS, KINDS)                                                                                                    \
+    asm volatile("{ .reg .pred e, p; setp.ne.b32 p, %6, 0; setp.ne.b32 e, %7, 0; @e tcgen05.mma.cta_group::" CGS ".kind::" KINDS     \
+                 " [%0], %1, %2, %3, [%4], [%5], p; }" ::"r"(d),                                                                      \
+                 "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc), "r"(e)                                                     \
                  : "memory")
     if constexpr (KIND == kKindBf16) {
         if constexpr (CG == 2) TKQ_MMA_PLAIN("2", "f16");
@@ -170,21 +201,31 @@ __device__ __forceinline__ void tcgen05_mma(uint32_t d, uint64_t a, uint64_t b, 
 // 512 bytes of scales (32 rows of 16 bytes) -> 4 columns x 32 lanes, repeated for the four lane quarters.  With CG = 2
 // each CTA of the pair copies from its own shared memory into its own tensor memory.
 template <int CG>
-__device__ __forceinline__ void tcgen05_copy_scales(uint32_t taddr, uint64_t desc) {
-    if constexpr (CG == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void tcgen05_copy_scales(bool one, uint32_t taddr, uint64_t desc) {
+    const uint32_t e = one ? 1u : 0u;
+    if constexpr (CG == 2)
+        asm volatile("{ .reg .pred e; setp.ne.b32 e, %2, 0; @e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1; }" ::"r"(taddr), "l"(desc), "r"(e)
+                     : "memory");
+    else
+        asm volatile("{ .reg .pred e; setp.ne.b32 e, %2, 0; @e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1; }" ::"r"(taddr), "l"(desc), "r"(e)
+                     : "memory");
 }
 
 // One arrival at `bar` (CG = 2: at the same barrier of both CTAs of the pair) once every tcgen05 operation this thread
 // has issued so far is complete.
 template <int CG>
-__device__ __forceinline__ void tcgen05_commit(uint32_t bar) {
+__device__ __forceinline__ void tcgen05_commit(bool one, uint32_t bar) {
+    const uint32_t e = one ? 1u : 0u;
     if constexpr (CG == 2)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-                     "h"(static_cast<uint16_t>(3))
-                     : "memory");
+        asm volatile(
+            "{ .reg .pred e; setp.ne.b32 e, %2, 0; @e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], "
+            "%1; }" ::"r"(bar),
+            "h"(static_cast<uint16_t>(3)), "r"(e)
+            : "memory");
     else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+        asm volatile("{ .reg .pred e; setp.ne.b32 e, %1, 0; @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar),
+                     "r"(e)
+                     : "memory");
 }
 
 }  // namespace tkq
