@@ -25,16 +25,15 @@ struct Operand {
     bool bf16;
 };
 
-static int encode(CUtensorMap* map, const Operand& o, uint32_t box_inner, uint32_t box_rows, bool fp32_out = false) {
+static int encode(CUtensorMap* map, const Operand& o, uint32_t box_inner, uint32_t box_rows) {
     auto fn = tensor_map_encoder();
     if (fn == nullptr) return set_error(TKQ_E_UNSUPPORTED, "cuTensorMapEncodeTiled is not available from this driver");
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(o.inner), static_cast<cuuint64_t>(o.rows), static_cast<cuuint64_t>(o.groups)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.row_bytes), static_cast<cuuint64_t>(o.group_bytes)};
     const cuuint32_t box[3] = {box_inner, box_rows, 1};
     const cuuint32_t steps[3] = {1, 1, 1};
-    const CUtensorMapDataType type = fp32_out ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : o.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    const CUresult r = fn(map, type, 3, const_cast<void*>(o.base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          fp32_out ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const CUresult r = fn(map, o.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(o.base), dims,
+                          strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(TKQ_E_UNSUPPORTED, "cuTensorMapEncodeTiled rejected an operand (alignment or size)");
     return 0;
@@ -50,17 +49,10 @@ static bool fix_strides(Operand& o) {
 
 template <class C>
 static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const char* what, cudaStream_t stream) {
-    alignas(64) CUtensorMap map_a, map_b, map_out{};
+    alignas(64) CUtensorMap map_a, map_b;
     if (int rc = encode(&map_a, a, C::A_MN ? 64 : C::kElems, C::A_MN ? 64 : 128)) return rc;
     if (int rc = encode(&map_b, b, C::WGRAD ? 64 : C::kElems, C::WGRAD ? 64 : C::kBRows)) return rc;
-    if (C::WGRAD && p.out_f32) {
-        const Operand o{p.out, p.i_size, p.j_size, p.groups, p.out_stride * 4, p.out_group_stride * 4, false};
-        p.wide_out = o.row_bytes % 16 == 0 && aligned16(o.base);
-        if (p.wide_out)
-            if (int rc = encode(&map_out, o, 32, 16, true)) return rc;
-    } else {
-        p.wide_out = p.i_size % 8 == 0 && p.out_stride % 8 == 0 && p.out_group_stride % 8 == 0 && aligned16(p.out);
-    }
+    p.wide_out = p.i_size % 8 == 0 && p.out_stride % 8 == 0 && p.out_group_stride % 8 == 0 && aligned16(p.out);
     p.i_tiles = (p.i_size + 128 * C::CG - 1) / (128 * C::CG);
     const int64_t j_tiles = C::WGRAD ? int64_t{p.groups} * ((p.j_size + C::NMAX - 1) / C::NMAX) : int64_t{p.rows} / C::NMAX + p.groups;
     if (j_tiles * p.i_tiles >= (int64_t{1} << 31)) return set_error(TKQ_E_UNSUPPORTED, "matrix product: more than 2^31 tiles");
@@ -79,7 +71,7 @@ static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const c
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = C::CG > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, map_a, map_b, map_out, p);
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, map_a, map_b, p);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return set_error(static_cast<int>(e), cudaGetErrorString(e));

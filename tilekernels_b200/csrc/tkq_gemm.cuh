@@ -55,7 +55,7 @@ struct GemmParams {
     uint32_t k_stages, last_units;  // forward: stages along K, matrix instructions of the last one
     uint32_t alpha_stride;
     uint32_t out_f32, accumulate, zero_gaps;
-    uint32_t wide_out;  // bf16: rows of out on 16-byte boundaries and i_size a multiple of 8; fp32: map_out is set
+    uint32_t wide_out;  // rows of out on 16-byte boundaries and i_size a multiple of 8
 };
 
 template <int KIND_, int CG_, int NMAX_, bool WGRAD_, bool A_MN_>
@@ -72,7 +72,7 @@ struct GemmConfig {
     static constexpr uint32_t kSfaBytes = 512 * kWords, kSfbBytes = 512 * kWords * kSfbBlocks;
     static constexpr uint32_t kStageBytes = kSub * (kABytes + kBBytes + kSfaBytes + kSfbBytes);
     static constexpr uint32_t kLoaders = SCALED ? 6 : 2;  // warps between the two issuing ones and those that store results
-    static constexpr uint32_t kFirstResultWarp = 2 + kLoaders, kResultWarps = SCALED ? 4 : 8;
+    static constexpr uint32_t kFirstResultWarp = 2 + kLoaders, kResultWarps = 4;
     static constexpr uint32_t kThreads = 32 * (kFirstResultWarp + kResultWarps);
     static constexpr uint32_t kStagingPerWarp = SCALED ? 2048 : 4096, kStagingBytes = kStagingPerWarp * kResultWarps;
     static constexpr uint32_t kFits = (kGemmSmemBudget - kStagingBytes) / kStageBytes;
@@ -287,11 +287,12 @@ __device__ __forceinline__ void store_bf16(const GemmParams& p, const GemmTile& 
     }
 }
 
-// The same for fp32 results of the weight gradient: rows of 128 bytes in shared memory leave by TMA, 16 rows at a time,
-// cut off at the tensor's edges; an accumulating call has them added in L2 (each element once).
+// fp32 results of the weight gradient: a warp's 32 lanes hold 32 neighbouring columns, 128 bytes of a row, so every store
+// is a whole line as it is.  (Shared memory is what the products are short of: staged rows and TMA stores took 600 us where
+// these take MEASURE, 16 experts, 8192 rows, 4096 x 7168.)  An accumulating call adds in L2, each element once.
 template <class C>
-__device__ __forceinline__ void store_f32(const GemmParams& p, const CUtensorMap& map_out, const GemmTile& tile, uint32_t (&v)[32], bool have,
-                                          uint32_t taddr, uint32_t iw, uint32_t c, uint32_t n, uint32_t smem, uint32_t& turn, uint32_t lane) {
+__device__ __forceinline__ void store_f32(const GemmParams& p, const GemmTile& tile, uint32_t (&v)[32], bool have, uint32_t taddr, uint32_t iw,
+                                          uint32_t c, uint32_t n, uint32_t lane) {
     if (have) {
         tmem_load32(taddr, v);
         tmem_load_wait();
@@ -299,37 +300,29 @@ __device__ __forceinline__ void store_f32(const GemmParams& p, const CUtensorMap
 #pragma unroll
         for (int q = 0; q < 32; ++q) v[q] = 0;
     }
-    if (p.wide_out) {
+    float* o = static_cast<float*>(p.out) + static_cast<int64_t>(tile.e) * p.out_group_stride + static_cast<int64_t>(tile.j0 + c) * p.out_stride + iw + lane;
+    if (iw + lane >= p.i_size) return;
+    if (n == 32 && !p.accumulate) {
 #pragma unroll
-        for (uint32_t half = 0; half < 2; ++half) {
-            const uint32_t buf = smem + (turn & 1u) * 2048u;
-            if (lane == 0) bulk_store_wait_read<1>();  // the store before the last one has left this half
-            __syncwarp();
-#pragma unroll
-            for (uint32_t q = 0; q < 16; ++q) asm volatile("st.shared.b32 [%0], %1;" ::"r"(buf + q * 128u + lane * 4u), "r"(v[16 * half + q]) : "memory");
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0 && iw < p.i_size && 16 * half < n)
-                tma_store_3d(&map_out, buf, static_cast<int32_t>(iw), static_cast<int32_t>(tile.j0 + c + 16 * half), static_cast<int32_t>(tile.e),
-                             p.accumulate != 0);
-            if (lane == 0) bulk_store_commit();
-            ++turn;
+        for (uint32_t q = 0; q < 32; ++q) {
+            asm volatile("st.global.L1::no_allocate.b32 [%0], %1;" ::"l"(o), "r"(v[q]) : "memory");
+            o += p.out_stride;
         }
-    } else if (iw + lane < p.i_size) {
-        float* o = static_cast<float*>(p.out) + static_cast<int64_t>(tile.e) * p.out_group_stride + static_cast<int64_t>(tile.j0 + c) * p.out_stride + iw + lane;
+    } else {
 #pragma unroll
-        for (uint32_t q = 0; q < 32; ++q)
+        for (uint32_t q = 0; q < 32; ++q) {
             if (q < n) {
-                float* at = o + static_cast<int64_t>(q) * p.out_stride;
-                *at = p.accumulate ? __fadd_rn(*at, __uint_as_float(v[q])) : __uint_as_float(v[q]);
+                if (p.accumulate) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(o), "f"(__uint_as_float(v[q])) : "memory");
+                else *o = __uint_as_float(v[q]);
             }
+            o += p.out_stride;
+        }
     }
 }
 
 template <class C>
 __global__ void __launch_bounds__(C::kThreads, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out,
-                const GemmParams p) {
+    gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full_bar[C::kStages], empty_bar[C::kStages], ready_bar[C::kStages], acc_full[2], acc_empty[2], drain_bar;
     __shared__ uint32_t tmem_slot;
@@ -446,6 +439,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                             for (uint32_t q = 0; q < C::kBRows / 64; ++q)
                                 tma_load_3d<C::CG>(b + q * 8192, &map_b, j0 + static_cast<int32_t>(64 * q), ku, 0, full);
                         } else {
+                            // (one box: the same rows in boxes of 32 took bf16 products from 312 to 360 us)
                             tma_load_3d<C::CG>(b + u * C::kBBytes, &map_b, ku, j0, 0, full);
                         }
                     }
@@ -636,7 +630,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 const uint32_t n = min(32u, tile.jn - c);
                 uint32_t v[32];
                 if (C::WGRAD && p.out_f32) {
-                    store_f32<C>(p, map_out, tile, v, have, taddr + c, iw, c, n, stage_mem, turn, lane);
+                    store_f32<C>(p, tile, v, have, taddr + c, iw, c, n, lane);
                 } else {
                     store_bf16<C>(p, tile, v, have, taddr + c, iw, c, n, alpha, stage_mem + (turn & 1u) * 2048u, lane);
                     if (C::kStagingPerWarp > 2048) ++turn;
@@ -649,7 +643,6 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 if (lane == 0) mbar_arrive_cluster(leader_bar(&acc_empty[a]));
             }
         }
-        if (C::WGRAD && lane == 0) bulk_store_wait_all();
         if (!C::WGRAD && p.zero_gaps) {
             // rows of no group: before the first, between two, behind the last
             const uint32_t w0 = blockIdx.x * C::kResultWarps + rw, nw = gridDim.x * C::kResultWarps;

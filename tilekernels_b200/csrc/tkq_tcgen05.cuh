@@ -67,21 +67,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
             : "memory");
 }
 
-// Tile store (or addition, in L2) of a box in shared memory; what lies outside the tensor is left out.  Coordinates are not
-// negative, x * element size a multiple of 16 bytes.
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* tmap, uint32_t smem_src, int32_t x, int32_t y, int32_t z, bool add) {
-    if (add)
-        asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tmap), "r"(x), "r"(y),
-                     "r"(z), "r"(smem_src)
-                     : "memory");
-    else
-        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tmap), "r"(x), "r"(y), "r"(z),
-                     "r"(smem_src)
-                     : "memory");
-}
-
-__device__ __forceinline__ void bulk_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-
 // ---------------------------------------------------------------------------
 // Tensor memory
 // ---------------------------------------------------------------------------
