@@ -5,18 +5,18 @@ from typing import Optional, Union
 import torch
 
 from .. import _lib
-from ..quant.block_scaled_gemm_kernel import check_out, launch_block_scaled_gemm, scaled_operand
+from ..quant.block_scaled_gemm_kernel import ScaledOperand, check_out, launch_block_scaled_gemm
 from ..quant.common import DTYPE_TO_ENUM, current_stream_ptr, device_guard
 from ..quant.types import QuantTensor
 
 
-def _check_groups(expert_start: torch.Tensor, expert_end: torch.Tensor, num_experts: int, device: torch.device) -> None:
+def _check_groups(expert_start: torch.Tensor, expert_end: torch.Tensor, num_experts: int, like: torch.Tensor) -> None:
     for t in (expert_start, expert_end):
-        assert t.dtype == torch.int32 and t.device == device and t.is_contiguous() and tuple(t.shape) == (num_experts,)
+        assert t.dtype is torch.int32 and t.get_device() == like.get_device() and t.shape == (num_experts,) and t.is_contiguous()
 
 
 def _check_matrix(x: torch.Tensor, dim: int) -> None:
-    assert x.dtype == torch.bfloat16 and x.is_cuda and x.dim() == dim
+    assert x.dtype is torch.bfloat16 and x.is_cuda and x.dim() == dim
     assert x.shape[-1] <= 1 or x.stride(-1) == 1
 
 
@@ -50,35 +50,37 @@ def grouped_gemm(
     Returns: (num_rows, n) bfloat16; fp32 sums, one rounding.
     """
     flags = _lib.ZERO_GAPS if out is None else 0
-    if isinstance(x, tuple):
+    quantized = isinstance(x, tuple)
+    if quantized:
         assert isinstance(w, tuple) and x_block_size is not None and w_block_size is not None
         assert not transpose_w, 'quantized weights are scaled along k: quantize the transposed weight instead'
         num_experts = w[0].shape[0]
-        xo, wo = scaled_operand(x, x_block_size, None), scaled_operand(w, w_block_size, num_experts)
-        num_rows, n, device = xo['rows'], wo['rows'], xo['data'].device
-        assert num_experts >= 1 and xo['k'] > 0 and xo['k'] == wo['k'], f"inner sizes differ: {xo['k']} and {wo['k']}"
-        assert wo['data'].device == device
+        xo, wo = ScaledOperand(x, x_block_size, None), ScaledOperand(w, w_block_size, num_experts)
+        num_rows, n, like = xo.rows, wo.rows, xo.data
     else:
         assert isinstance(w, torch.Tensor) and x_block_size is None and w_block_size is None and alpha is None
         _check_matrix(x, 2)
         _check_matrix(w, 3)
-        assert w.device == x.device
         num_experts, n, k = (w.shape[0], w.shape[2], w.shape[1]) if transpose_w else w.shape
-        num_rows, device = x.shape[0], x.device
-        assert num_experts >= 1 and k > 0 and x.shape[1] == k, f'inner sizes differ: {x.shape[1]} and {k}'
-    _check_groups(expert_start, expert_end, num_experts, device)
+        num_rows, like = x.shape[0], x
+        assert w.get_device() == x.get_device()
+        assert k > 0 and x.shape[1] == k, f'inner sizes differ: {x.shape[1]} and {k}'
+    assert num_experts >= 1
+    _check_groups(expert_start, expert_end, num_experts, like)
+    device = like.device
     if out is None:
         out = torch.empty((num_rows, n), dtype=torch.bfloat16, device=device)
     else:
-        check_out(out, (num_rows, n), torch.bfloat16, device)
-    if isinstance(x, tuple):
+        check_out(out, (num_rows, n), like)
+    if quantized:
         launch_block_scaled_gemm(xo, wo, expert_start, expert_end, num_experts, alpha, out, flags)
     elif num_rows > 0 and n > 0:
         with device_guard(device):
             rc = _lib.lib().tkq_grouped_gemm(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w.stride(1), int(transpose_w),
                                              expert_start.data_ptr(), expert_end.data_ptr(), num_experts, num_rows, n, k, out.data_ptr(),
                                              out.stride(0), flags, current_stream_ptr(device))
-        _lib.check(rc, 'tkq_grouped_gemm')
+        if rc:
+            _lib.check(rc, 'tkq_grouped_gemm')
     return out
 
 
@@ -105,23 +107,24 @@ def grouped_gemm_wgrad(
     """
     _check_matrix(grad, 2)
     _check_matrix(x, 2)
-    device = x.device
-    assert grad.device == device and grad.shape[0] == x.shape[0]
-    assert out_dtype in (torch.float32, torch.bfloat16)
+    assert grad.get_device() == x.get_device() and grad.shape[0] == x.shape[0]
+    assert out_dtype is torch.float32 or out_dtype is torch.bfloat16
     num_rows, n, k = x.shape[0], grad.shape[1], x.shape[1]
     num_experts = expert_start.numel()
     assert num_experts >= 1
-    _check_groups(expert_start, expert_end, num_experts, device)
+    _check_groups(expert_start, expert_end, num_experts, x)
+    device = x.device
     if out is None:
         assert not accumulate, 'accumulate needs out'
         out = torch.empty((num_experts, n, k), dtype=out_dtype, device=device)
     else:
-        assert tuple(out.shape) == (num_experts, n, k) and out.dtype == out_dtype and out.device == device and out.is_contiguous()
-        assert not accumulate or out_dtype == torch.float32, 'accumulate needs a float32 destination'
+        assert out.shape == (num_experts, n, k) and out.dtype is out_dtype and out.get_device() == x.get_device() and out.is_contiguous()
+        assert not accumulate or out_dtype is torch.float32, 'accumulate needs a float32 destination'
     if n > 0 and k > 0:
         with device_guard(device):
             rc = _lib.lib().tkq_grouped_gemm_wgrad(grad.data_ptr(), grad.stride(0), x.data_ptr(), x.stride(0), expert_start.data_ptr(),
                                                    expert_end.data_ptr(), num_experts, num_rows, n, k, DTYPE_TO_ENUM[out_dtype],
                                                    out.data_ptr(), _lib.ACCUMULATE if accumulate else 0, current_stream_ptr(device))
-        _lib.check(rc, 'tkq_grouped_gemm_wgrad')
+        if rc:
+            _lib.check(rc, 'tkq_grouped_gemm_wgrad')
     return out

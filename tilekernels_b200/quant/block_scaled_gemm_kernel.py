@@ -5,79 +5,86 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .common import FMT_TO_ENUM, current_stream_ptr, device_guard, get_logical_hidden
+from .common import current_stream_ptr, device_guard
 from .types import QuantTensor
 
 
-def scaled_operand(x: QuantTensor, block_size: tuple[int, int], num_groups: Optional[int]) -> dict:
-    """Checks a quantized operand and describes it for tkq_block_scaled_gemm.  `num_groups` None: a matrix
-    (rows, k); else stacked matrices (num_groups, rows, k), whose scales may also come as one matrix of all rows."""
-    data, sf = x
-    assert isinstance(data, torch.Tensor) and isinstance(sf, torch.Tensor)
-    assert data.dtype in (torch.float8_e4m3fn, torch.int8), 'data is float8_e4m3fn or int8 (two FP4 per byte)'
-    assert data.is_cuda and sf.is_cuda and sf.device == data.device
-    block_m, block_k = block_size
-    rows = data.shape[-2]
-    k = get_logical_hidden(data.shape[-1], data.dtype)
-    assert data.dim() == (2 if num_groups is None else 3) and (data.shape[-1] <= 1 or data.stride(-1) == 1)
-    assert block_m in (1, 32, 128)
-    blocks = -(-rows // block_m)
-    if sf.dtype == torch.float8_e4m3fn:
-        # one e4m3 scale per 16 values, four bytes read at a time: the scales of a row lie together
-        assert data.dtype == torch.int8 and block_k == 16 and block_m == 1, 'float8_e4m3fn scales go with FP4 data and blocks of (1, 16)'
-        assert k % 64 == 0 and sf.stride(-1) == 1
-        sf = sf.view(torch.int32)
-    else:
-        assert sf.dtype == torch.int32, 'scales are packed ue8m0 words (int32) or float8_e4m3fn'
-        assert block_k in ((32, 128) if data.dtype == torch.float8_e4m3fn else (32,))
-    words = -(-k // (4 * block_k))
-    if num_groups is None:
-        assert tuple(sf.shape) == (blocks, words), f'scales must be {(blocks, words)}, got {tuple(sf.shape)}'
-        sf_strides = (0,) + sf.stride()
-    elif sf.dim() == 3:
-        assert tuple(sf.shape) == (num_groups, blocks, words), f'scales must be {(num_groups, blocks, words)}, got {tuple(sf.shape)}'
+class ScaledOperand:
+    """A checked quantized operand as tkq_block_scaled_gemm takes it: a matrix (rows, k), or with `num_groups` stacked
+    matrices (num_groups, rows, k), whose scales may also come as one matrix of all rows."""
+    __slots__ = ('data', 'sf', 'rows', 'k', 'block_m', 'block_k', 'fmt', 'sf_fmt', 'group_stride', 'row_stride', 'sf_strides')
+
+    def __init__(self, x: QuantTensor, block_size: tuple[int, int], num_groups: Optional[int]):
+        data, sf = x
+        block_m, block_k = block_size
+        assert data.is_cuda and sf.is_cuda and data.get_device() == sf.get_device()
+        assert data.dim() == (2 if num_groups is None else 3)
+        shape, strides = data.shape, data.stride()
+        rows, physical = shape[-2], shape[-1]
+        assert physical <= 1 or strides[-1] == 1
+        assert block_m in (1, 32, 128)
+        if data.dtype is torch.float8_e4m3fn:
+            per_byte, self.fmt, k = 1, _lib.FMT_E4M3, physical
+        else:
+            assert data.dtype is torch.int8, 'data is float8_e4m3fn or int8 (two FP4 per byte)'
+            per_byte, self.fmt, k = 2, _lib.FMT_E2M1, physical * 2
+        blocks = rows if block_m == 1 else -(-rows // block_m)
+        if sf.dtype is torch.float8_e4m3fn:
+            # one e4m3 scale per 16 values, four bytes read at a time: the scales of a row lie together
+            assert per_byte == 2 and block_k == 16 and block_m == 1, 'float8_e4m3fn scales go with FP4 data and blocks of (1, 16)'
+            assert k % 64 == 0 and sf.stride(-1) == 1
+            sf = sf.view(torch.int32)
+            self.sf_fmt = _lib.SFMT_E4M3
+        else:
+            assert sf.dtype is torch.int32, 'scales are packed ue8m0 words (int32) or float8_e4m3fn'
+            assert block_k == 32 or (block_k == 128 and per_byte == 1)
+            self.sf_fmt = _lib.SFMT_UE8M0
+        words = -(-k // (4 * block_k))
         sf_strides = sf.stride()
-    else:
-        assert rows % block_m == 0, 'scales of all groups in one matrix need whole blocks of rows per group'
-        assert tuple(sf.shape) == (num_groups * blocks, words), f'scales must be {(num_groups * blocks, words)}, got {tuple(sf.shape)}'
-        sf_strides = (blocks * sf.stride(0),) + sf.stride()
-    per_byte = 2 if data.dtype == torch.int8 else 1
-    return dict(data=data, sf=sf, rows=rows, k=k, block=(block_m, block_k), fmt='e2m1' if data.dtype == torch.int8 else 'e4m3',
-                sf_fmt=_lib.SFMT_E4M3 if block_k == 16 else _lib.SFMT_UE8M0, strides=tuple(per_byte * s for s in data.stride()[:-1]),
-                sf_strides=sf_strides)
+        if num_groups is None:
+            assert sf.shape == (blocks, words), f'scales must be {(blocks, words)}, got {tuple(sf.shape)}'
+            self.sf_strides = (0,) + sf_strides
+            self.group_stride = 0
+        else:
+            if len(sf_strides) == 3:
+                assert sf.shape == (num_groups, blocks, words), f'scales must be {(num_groups, blocks, words)}, got {tuple(sf.shape)}'
+                self.sf_strides = sf_strides
+            else:
+                assert rows % block_m == 0, 'scales of all groups in one matrix need whole blocks of rows per group'
+                assert sf.shape == (num_groups * blocks, words), f'scales must be {(num_groups * blocks, words)}, got {tuple(sf.shape)}'
+                self.sf_strides = (blocks * sf_strides[0],) + sf_strides
+            self.group_stride = per_byte * strides[0]
+        self.data, self.sf, self.rows, self.k, self.block_m, self.block_k = data, sf, rows, k, block_m, block_k
+        self.row_stride = per_byte * strides[-2]
 
 
-def check_alpha(alpha: Optional[torch.Tensor], device: torch.device, count: int) -> tuple[Optional[int], int]:
-    """Pointer and stride of the optional fp32 factors: one for all, or `count`."""
-    if alpha is None:
-        return None, 0
-    assert alpha.dtype == torch.float32 and alpha.device == device and alpha.numel() in (1, count)
-    assert alpha.dim() <= 1
-    return alpha.data_ptr(), alpha.stride(0) if alpha.numel() > 1 else 0
+def check_out(out: torch.Tensor, shape: tuple, like: torch.Tensor) -> None:
+    assert out.dim() == 2 and out.shape == shape and out.dtype is torch.bfloat16 and out.get_device() == like.get_device()
+    assert (shape[1] <= 1 or out.stride(1) == 1) and (shape[0] <= 1 or out.stride(0) >= shape[1])
 
 
-def check_out(out: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
-    assert out.shape == shape and out.dtype == dtype and out.device == device
-    assert out.dim() == 2 and (out.shape[1] <= 1 or out.stride(1) == 1) and (out.shape[0] <= 1 or out.stride(0) >= out.shape[1])
-
-
-def launch_block_scaled_gemm(x: dict, w: dict, expert_start, expert_end, num_experts: int, alpha, out: torch.Tensor, flags: int) -> None:
-    assert x['k'] == w['k'], f"inner sizes differ: {x['k']} and {w['k']}"
-    assert x['fmt'] == w['fmt'] and x['sf_fmt'] == w['sf_fmt'], 'both operands must have the same format'
-    assert x['data'].device == w['data'].device
-    num_rows, n, k = x['rows'], w['rows'], x['k']
-    alpha_ptr, alpha_stride = check_alpha(alpha, x['data'].device, num_experts)
-    w_strides = w['strides'] if len(w['strides']) == 2 else (0,) + w['strides']
-    if num_rows == 0 or n == 0:
+def launch_block_scaled_gemm(x: ScaledOperand, w: ScaledOperand, expert_start, expert_end, num_experts: int, alpha, out: torch.Tensor,
+                             flags: int) -> None:
+    assert x.k > 0 and x.k == w.k, f'inner sizes differ: {x.k} and {w.k}'
+    assert x.fmt == w.fmt and x.sf_fmt == w.sf_fmt, 'both operands must have the same format'
+    assert x.data.get_device() == w.data.get_device()
+    alpha_ptr, alpha_stride = None, 0
+    if alpha is not None:
+        assert alpha.dtype is torch.float32 and alpha.get_device() == x.data.get_device() and alpha.dim() <= 1
+        assert alpha.numel() in (1, num_experts)
+        alpha_ptr = alpha.data_ptr()
+        alpha_stride = alpha.stride(0) if alpha.numel() > 1 else 0
+    if x.rows == 0 or w.rows == 0:
         return
-    with device_guard(out.device):
+    device = out.device
+    with device_guard(device):
         rc = _lib.lib().tkq_block_scaled_gemm(
-            x['data'].data_ptr(), x['strides'][-1], x['sf'].data_ptr(), x['sf_strides'][1], x['sf_strides'][2], x['block'][0],
-            x['block'][1], w['data'].data_ptr(), w_strides[0], w_strides[1], w['sf'].data_ptr(), *w['sf_strides'], w['block'][0],
-            w['block'][1], FMT_TO_ENUM[x['fmt']], x['sf_fmt'], None if expert_start is None else expert_start.data_ptr(),
-            None if expert_end is None else expert_end.data_ptr(), num_experts, num_rows, n, k, alpha_ptr, alpha_stride, out.data_ptr(),
-            out.stride(0), flags, current_stream_ptr(out.device))
-    _lib.check(rc, 'tkq_block_scaled_gemm')
+            x.data.data_ptr(), x.row_stride, x.sf.data_ptr(), x.sf_strides[1], x.sf_strides[2], x.block_m, x.block_k, w.data.data_ptr(),
+            w.group_stride, w.row_stride, w.sf.data_ptr(), *w.sf_strides, w.block_m, w.block_k, x.fmt, x.sf_fmt,
+            None if expert_start is None else expert_start.data_ptr(), None if expert_end is None else expert_end.data_ptr(),
+            num_experts, x.rows, w.rows, x.k, alpha_ptr, alpha_stride, out.data_ptr(), out.stride(0), flags, current_stream_ptr(device))
+    if rc:
+        _lib.check(rc, 'tkq_block_scaled_gemm')
 
 
 def block_scaled_gemm(
@@ -105,12 +112,11 @@ def block_scaled_gemm(
 
     Returns: (m, n) bfloat16.
     """
-    x, w = scaled_operand(a, a_block_size, None), scaled_operand(b, b_block_size, None)
-    assert x['k'] > 0 and x['k'] == w['k'], f"inner sizes differ: {x['k']} and {w['k']}"
-    shape = (x['rows'], w['rows'])
+    x, w = ScaledOperand(a, a_block_size, None), ScaledOperand(b, b_block_size, None)
+    shape = (x.rows, w.rows)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=x['data'].device)
+        out = torch.empty(shape, dtype=torch.bfloat16, device=x.data.device)
     else:
-        check_out(out, shape, torch.bfloat16, x['data'].device)
+        check_out(out, shape, x.data)
     launch_block_scaled_gemm(x, w, None, None, 1, alpha, out, 0)
     return out

@@ -9,7 +9,7 @@ from .types import QuantTensor
 
 def _check_tensor_scale(tensor_scale: torch.Tensor, device: torch.device) -> None:
     assert isinstance(tensor_scale, torch.Tensor), 'tensor_scale is a CUDA tensor: its value is read on the device'
-    assert tensor_scale.dtype == torch.float32 and tensor_scale.numel() == 1 and tensor_scale.device == device
+    assert tensor_scale.dtype is torch.float32 and tensor_scale.numel() == 1 and tensor_scale.get_device() == device.index
 
 
 def per_token_cast_to_nvfp4(x: torch.Tensor, tensor_scale: torch.Tensor) -> QuantTensor:
@@ -39,7 +39,8 @@ def per_token_cast_to_nvfp4(x: torch.Tensor, tensor_scale: torch.Tensor) -> Quan
         with device_guard(x.device):
             rc = _lib.lib().tkq_per_token_cast_nvfp4(x.data_ptr(), DTYPE_TO_ENUM[x.dtype], num_tokens, hidden, x.stride(0),
                                                      tensor_scale.data_ptr(), out.data_ptr(), out_sf.data_ptr(), current_stream_ptr(x.device))
-        _lib.check(rc, 'tkq_per_token_cast_nvfp4')
+        if rc:
+            _lib.check(rc, 'tkq_per_token_cast_nvfp4')
     return out, out_sf
 
 
@@ -49,12 +50,13 @@ def cast_back_nvfp4(x: QuantTensor, fmt: str, tensor_scale: torch.Tensor) -> tor
     assert data.dim() == 2 and data.dtype == torch.int8 and data.is_contiguous() and data.is_cuda
     num_tokens, hidden = data.shape[0], data.shape[1] * 2
     assert hidden > 0 and hidden % 16 == 0
-    assert sf.dtype == torch.float8_e4m3fn and tuple(sf.shape) == (num_tokens, hidden // 16) and sf.is_contiguous() and sf.device == data.device
+    assert sf.dtype == torch.float8_e4m3fn and sf.shape == (num_tokens, hidden // 16) and sf.is_contiguous() and sf.get_device() == data.get_device()
     _check_tensor_scale(tensor_scale, data.device)
     out = torch.empty((num_tokens, hidden), dtype=torch.bfloat16 if fmt == 'bf16' else torch.float32, device=data.device)
     if num_tokens > 0:
         with device_guard(data.device):
             rc = _lib.lib().tkq_cast_back_nvfp4(data.data_ptr(), sf.data_ptr(), tensor_scale.data_ptr(), num_tokens, hidden,
                                                 DTYPE_TO_ENUM[out.dtype], out.data_ptr(), current_stream_ptr(data.device))
-        _lib.check(rc, 'tkq_cast_back_nvfp4')
+        if rc:
+            _lib.check(rc, 'tkq_cast_back_nvfp4')
     return out
