@@ -54,6 +54,22 @@ def test_against_64_bits(cuda_device, form, m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('form', FORMS, ids=_id)
+@pytest.mark.parametrize('m,n,k', ((1, 200, 7168), (16, 8, 16384), (31, 129, 4096), (33, 264, 6400), (64, 1024, 3328), (65, 100, 12288)))
+def test_few_tiles_and_a_long_k(cuda_device, form, m, n, k):
+    """Products that several blocks share along k, down to the last columns of the last part."""
+    from tilekernels_b200 import quant
+    fmt, ab, bb = form
+    a, b = _matrices(m, n, k, cuda_device)
+    (qa, va, ta), (qb, vb, tb) = quantize(a, fmt, ab), quantize(b, fmt, bb)
+    alpha = ta * tb if fmt == 'nvfp4' else None
+    got = quant.block_scaled_gemm(qa, qb, ab, bb, alpha=alpha)
+    assert_product(got, va, vb, 1.0 if alpha is None else alpha.double().item())
+    for _ in range(3):
+        assert torch.equal(quant.block_scaled_gemm(qa, qb, ab, bb, alpha=alpha), got)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('m', (1, 300))
 def test_alpha_out_and_strides(cuda_device, m):
     from tilekernels_b200 import quant

@@ -53,6 +53,21 @@ def test_bf16(cuda_device, name, n, k, transpose):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('sizes', ((1,), (20,), (0, 3), (50,), (61, 0)))
+@pytest.mark.parametrize('transpose', (False, True), ids=('w', 'w_t'))
+def test_few_tiles_and_a_long_k(cuda_device, sizes, transpose):
+    """Products that several blocks share along k."""
+    from tilekernels_b200 import moe
+    n, k = 200, 3992
+    x, start, end, member = _rows(sizes, k, cuda_device)
+    gen = torch.Generator().manual_seed(n)
+    w = torch.randn((len(sizes), k, n) if transpose else (len(sizes), n, k), generator=gen).to(torch.bfloat16).to(cuda_device)
+    got = moe.grouped_gemm(x, w, int32(start, cuda_device), int32(end, cuda_device), transpose_w=transpose)
+    _check_groups(got, x.cpu().double(), w.cpu().double(), start, end, transpose)
+    assert (got[~member.to(cuda_device)] == 0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('name', SIZES)
 @pytest.mark.parametrize('form', (('e4m3', (1, 128), (128, 128)), ('e4m3', (1, 32), (1, 32)), ('e2m1', (1, 32), (1, 32)),
                                   ('nvfp4', (1, 16), (1, 16))), ids=lambda f: f'{f[0]}-{f[1][1]}')

@@ -56,21 +56,23 @@ static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const c
     p.i_tiles = (p.i_size + 128 * C::CG - 1) / (128 * C::CG);
     const int64_t j_tiles = C::WGRAD ? int64_t{p.groups} * ((p.j_size + C::NMAX - 1) / C::NMAX) : int64_t{p.rows} / C::NMAX + p.groups;
     if (j_tiles * p.i_tiles >= (int64_t{1} << 31)) return set_error(TKQ_E_UNSUPPORTED, "matrix product: more than 2^31 tiles");
-    const int64_t units = std::min<int64_t>(j_tiles * p.i_tiles, device_sm_count() / C::CG);
-    const int smem = static_cast<int>(1024 + C::kStages * C::kStageBytes + C::kStagingBytes + 4 * (3 * p.groups + 1));
+    // CTAs of a cluster: a pair on one tile, or those that share a tile along K
+    const int cluster = C::SPLIT ? static_cast<int>(p.split) : C::CG;
+    const int64_t units = std::min<int64_t>(j_tiles * p.i_tiles, device_sm_count() / cluster);
+    const int smem = static_cast<int>(1024 + C::kStages * C::kStageBytes + C::kStagingBytes + C::kPartialBytes + 4 * (3 * p.groups + 1));
     auto kernel = gemm_kernel<C>;
     if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(units * C::CG));
+    config.gridDim = dim3(static_cast<unsigned>(units * cluster));
     config.blockDim = dim3(C::kThreads);
     config.dynamicSmemBytes = static_cast<size_t>(smem);
     config.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = C::CG;
+    attr.val.clusterDim.x = cluster;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     config.attrs = &attr;
-    config.numAttrs = C::CG > 1 ? 1 : 0;
+    config.numAttrs = cluster > 1 ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&config, kernel, map_a, map_b, p);
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -79,12 +81,42 @@ static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const c
     return check_launch(what);
 }
 
-// Tile variant by the mean number of rows per group.
+// At most so many tiles along j: exact for one group, else with a partial tile in each.
+static int64_t row_tiles(const GemmParams& p, int nmax) {
+    return p.groups == 1 ? (int64_t{p.rows} + nmax - 1) / nmax : int64_t{p.rows} / nmax + p.groups;
+}
+
+// Tiles that leave most SMs idle are split along K, over as many CTAs as there are SMs for; a cluster takes one tile.  One
+// row of FP8 through 4096 x 7168: 14.9 us whole, 10.5 us split by 4; of NVFP4 through 7168 x 2048 (eight stages): 7.8 us
+// whole, 8.4 us split by 2, so a part has at least six stages.
+template <int KIND, int NMAX, bool A_MN>
+static bool launch_split(const Operand& a, const Operand& b, GemmParams p, const char* what, cudaStream_t stream, int* rc) {
+    const int64_t tiles = row_tiles(p, NMAX) * ((p.i_size + 127) / 128);
+    p.split = 1;
+    while (p.split < 8 && tiles * p.split * 2 <= device_sm_count() && p.k_stages >= 12 * p.split) p.split *= 2;
+    if (p.split == 1) return false;
+    *rc = launch_gemm<GemmConfig<KIND, 1, NMAX, false, A_MN, true>>(a, b, p, what, stream);
+    return true;
+}
+
+// Tile variant by the mean number of rows per group.  Measured (us; 32 groups, 4096 x 7168, MXFP4 and bf16):
+//   mean rows          20          34          64         100         200
+//   128 x 32        83, -     105, 372    146, 540    198, 746   358, 1394
+//   128 x 128       85, -      87, 287     93, 306    106, 361   148, 510
+//   pair x 224/256  88, -      90, 288     92, 294     97, 315   124, 406
+// One group whose smaller tiles all run at once uses more SMs with them (200 rows of MXFP4: 13.0 against 16.3 us for the
+// pair, 256 of FP8: 20.8 against 22.3).
 template <int KIND, int NMID, int NLARGE, bool A_MN>
 static int launch_rows(const Operand& a, const Operand& b, const GemmParams& p, const char* what, cudaStream_t stream) {
     const int64_t mean = p.rows / p.groups;
-    if (mean <= 32) return launch_gemm<GemmConfig<KIND, 1, 32, false, A_MN>>(a, b, p, what, stream);
-    if (mean <= 128) return launch_gemm<GemmConfig<KIND, 1, NMID, false, A_MN>>(a, b, p, what, stream);
+    int rc;
+    if (mean <= 32) {
+        if (launch_split<KIND, 32, A_MN>(a, b, p, what, stream, &rc)) return rc;
+        return launch_gemm<GemmConfig<KIND, 1, 32, false, A_MN>>(a, b, p, what, stream);
+    }
+    if (mean <= 128 && launch_split<KIND, 64, A_MN>(a, b, p, what, stream, &rc)) return rc;
+    if (mean <= 48 || row_tiles(p, NMID) * ((p.i_size + 127) / 128) <= device_sm_count())
+        return launch_gemm<GemmConfig<KIND, 1, NMID, false, A_MN>>(a, b, p, what, stream);
     return launch_gemm<GemmConfig<KIND, 2, NLARGE, false, A_MN>>(a, b, p, what, stream);
 }
 

@@ -16,6 +16,9 @@
 // layout the tensor core copies them from (or, for the weight gradient, clear the rows behind a group's end), warps 4 to
 // 7 store results.  Blocks are persistent and take tiles in turn.  With CG = 2 two CTAs on neighbouring SMs work on one
 // tile of 256 x N: each holds half of A's and half of B's rows, which halves the shared-memory fill per product.
+//
+// With few tiles (one token through one matrix) K is split over a cluster of CTAs: each multiplies its part of K, hands
+// its sums to the CTAs that own the columns, through their shared memory, and those add them in the order of the parts.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -54,14 +57,15 @@ struct GemmParams {
     uint32_t i_tiles;
     uint32_t k_stages, last_units;  // forward: stages along K, matrix instructions of the last one
     uint32_t alpha_stride;
+    uint32_t split;  // CTAs of a cluster that share a tile along K
     uint32_t out_f32, accumulate, zero_gaps;
     uint32_t wide_out;  // rows of out on 16-byte boundaries and i_size a multiple of 8
 };
 
-template <int KIND_, int CG_, int NMAX_, bool WGRAD_, bool A_MN_>
+template <int KIND_, int CG_, int NMAX_, bool WGRAD_, bool A_MN_, bool SPLIT_ = false>
 struct GemmConfig {
     static constexpr int KIND = KIND_, CG = CG_, NMAX = NMAX_;
-    static constexpr bool WGRAD = WGRAD_, A_MN = A_MN_, SCALED = KIND_ != kKindBf16;
+    static constexpr bool WGRAD = WGRAD_, A_MN = A_MN_, SCALED = KIND_ != kKindBf16, SPLIT = SPLIT_;
     // A stage holds kSub blocks of 128 bytes along K.  Waiting for a stage and handing it back costs the issuing warp some
     // 200 cycles: two thirds of a block's products in 4 or 8 bits (448 cycles at N = 224), which therefore come in pairs
     static constexpr uint32_t kSub = SCALED ? 2 : 1;
@@ -75,7 +79,8 @@ struct GemmConfig {
     static constexpr uint32_t kFirstResultWarp = 2 + kLoaders, kResultWarps = 4;
     static constexpr uint32_t kThreads = 32 * (kFirstResultWarp + kResultWarps);
     static constexpr uint32_t kStagingPerWarp = SCALED ? 2048 : 4096, kStagingBytes = kStagingPerWarp * kResultWarps;
-    static constexpr uint32_t kFits = (kGemmSmemBudget - kStagingBytes) / kStageBytes;
+    static constexpr uint32_t kPartialBytes = SPLIT ? NMAX * 128 * 4 : 0;
+    static constexpr uint32_t kFits = (kGemmSmemBudget - kStagingBytes - kPartialBytes) / kStageBytes;
     static constexpr uint32_t kStages = kFits < 10 ? kFits : 10;
     static constexpr uint32_t kSfCols = 4 * kWords * (1 + kSfbBlocks);  // tensor-memory columns of one block's scales
     static constexpr uint32_t kSfBase = 2 * NMAX;
@@ -85,8 +90,12 @@ struct GemmConfig {
     static constexpr uint32_t kNStep = CG == 2 ? 32 : 16;
     static_assert(kColsNeeded <= 512, "tensor memory");
     static_assert(kFirstResultWarp % 4 == 0, "a warp reads the quarter of tensor memory of its number modulo four");
+    static_assert(!SPLIT || (CG == 1 && !WGRAD), "the cluster of a split product is one along K");
     static_assert(!WGRAD || (A_MN && kBRows % 64 == 0 && kSub == 1), "weight gradient reads both operands along their rows");
-    static_assert(kBBytes % 1024 == 0 && kStages >= 3, "stage layout");
+    static_assert(kBBytes % 1024 == 0, "stage layout");
+    // A scale loader goes from stage `it` to `it` + 3.  It waits by parity, so the slot it comes to has to be at most one phase
+    // behind: MMA(it - kStages) is done by then, MMA(it + 3 - 2 kStages) has to be.
+    static_assert(kStages >= 3 && kStages >= kLoaders / 2, "a slot's parity would be ambiguous");
 };
 
 struct GemmTile {
@@ -213,17 +222,21 @@ struct ScaleWalk {
     uint32_t t, stage, it;
     bool valid;
 
-    __device__ __forceinline__ void begin(const GemmParams& p, const GemmSchedule<C>& sched, uint32_t unit) {
+    uint32_t first, last;  // the block's part of K
+
+    __device__ __forceinline__ void begin(const GemmParams& p, const GemmSchedule<C>& sched, uint32_t unit, uint32_t k_first, uint32_t k_end) {
         t = unit;
-        stage = it = 0;
+        first = stage = k_first;
+        last = k_end;
+        it = 0;
         valid = t < sched.total;
         if (valid) tile = sched.tile(p, t);
     }
     __device__ __forceinline__ void advance(const GemmParams& p, const GemmSchedule<C>& sched, uint32_t units, uint32_t stages) {
         stage += stages;
         it += stages;
-        while (valid && stage >= p.k_stages) {
-            stage -= p.k_stages;
+        while (valid && stage >= last) {
+            stage -= last - first;
             t += units;
             valid = t < sched.total;
             if (valid) tile = sched.tile(p, t);
@@ -330,12 +343,17 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = C::CG == 2 ? cluster_rank() : 0;
-    const uint32_t unit = blockIdx.x / C::CG, units = gridDim.x / C::CG;
+    const uint32_t unit = blockIdx.x / (C::SPLIT ? p.split : C::CG), units = gridDim.x / (C::SPLIT ? p.split : C::CG);
+    // this CTA's part of K
+    const uint32_t part = C::SPLIT ? cluster_rank() : 0;
+    const uint32_t k_first = C::SPLIT ? part * p.k_stages / p.split : 0;
+    const uint32_t k_end = C::SPLIT ? (part + 1) * p.k_stages / p.split : p.k_stages;
 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t a_base = base, b_base = a_base + C::kStages * C::kSub * C::kABytes, staging = b_base + C::kStages * C::kSub * C::kBBytes;
-    const uint32_t sf_base = staging + C::kStagingBytes;
-    uint32_t* group_mem = reinterpret_cast<uint32_t*>(smem_raw + (base - smem_u32(smem_raw)) + C::kStages * C::kStageBytes + C::kStagingBytes);
+    const uint32_t partial = staging + C::kStagingBytes, sf_base = partial + C::kPartialBytes;
+    uint32_t* group_mem =
+        reinterpret_cast<uint32_t*>(smem_raw + (base - smem_u32(smem_raw)) + C::kStages * C::kStageBytes + C::kStagingBytes + C::kPartialBytes);
     uint32_t* s_prefix = group_mem;
     uint32_t* s_start = s_prefix + p.groups + 1;
     uint32_t* s_rows = s_start + p.groups;
@@ -391,7 +409,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     }
     tcgen05_fence_before();
     __syncthreads();
-    if constexpr (C::CG == 2) cluster_sync();
+    if constexpr (C::CG == 2 || C::SPLIT) cluster_sync();  // (a split product's CTAs write to one another)
     tcgen05_fence_after();
 
     const uint32_t tmem = tmem_slot;
@@ -414,8 +432,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             const GemmTile tile = sched.tile(p, t);
             const int32_t i0 = static_cast<int32_t>(tile.i0 + rank * 128u);
             const int32_t j0 = static_cast<int32_t>(tile.j0 + (C::CG == 2 ? rank * (tile.n_mma / 2) : 0));
-            const uint32_t k_stages = C::WGRAD ? tile.k_stages : p.k_stages;
-            for (uint32_t kb = 0; kb < k_stages; ++kb) {
+            const uint32_t k_last = C::WGRAD ? tile.k_stages : k_end;
+            for (uint32_t kb = k_first; kb < k_last; ++kb) {
                 ok = __any_sync(kFullMask, one && wait(bar(&empty_bar[s]), phase));
                 if (!ok) break;
                 const uint32_t a = a_base + s * (C::kSub * C::kABytes), b = b_base + s * (C::kSub * C::kBBytes);
@@ -474,8 +492,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             bool ok = true, ready = false;  // ready: the next stage's operands have been seen to be there
             for (uint32_t t = unit; ok && t < sched.total; t += units) {
                 const GemmTile tile = sched.tile(p, t);
-                const uint32_t k_stages = C::WGRAD ? tile.k_stages : p.k_stages;
-                if (k_stages == 0) continue;
+                const uint32_t k_last = C::WGRAD ? tile.k_stages : k_end;
+                if (k_last == 0) continue;
                 const uint32_t a = acc_it & 1u;
                 ok = __any_sync(kFullMask, one && wait(bar(&acc_empty[a]), ((acc_it >> 1) & 1u) ^ 1u));
                 if (!ok) break;
@@ -485,7 +503,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 uint32_t idesc;
                 if constexpr (C::SCALED) idesc = idesc_scaled(kM, tile.n_mma, C::KIND == kKindMxf8 ? 0 : 1, C::KIND != kKindNvf4);
                 else idesc = idesc_bf16(kM, tile.n_mma, C::A_MN, C::WGRAD);
-                for (uint32_t kb = 0; kb < k_stages; ++kb) {
+                for (uint32_t kb = k_first; kb < k_last; ++kb) {
                     if (!ready) ok = __any_sync(kFullMask, one && wait(bar(C::WGRAD ? &ready_bar[s] : &full_bar[s]), phase));
                     if (!ok) break;
                     tcgen05_fence_after();
@@ -494,7 +512,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                     bool seen = false;
                     if (one) seen = mbar_try_wait_cluster(bar(C::WGRAD ? &ready_bar[s] : &full_bar[s]), phase);
                     uint32_t n_units = 4 * C::kSub;
-                    if (kb + 1 == k_stages) n_units = C::WGRAD ? (tile.k_rows - kb * 64 + 15) / 16 : p.last_units;
+                    if (kb + 1 == (C::WGRAD ? k_last : p.k_stages)) n_units = C::WGRAD ? (tile.k_rows - kb * 64 + 15) / 16 : p.last_units;
 #pragma unroll
                     for (uint32_t h = 0; h < C::kSub; ++h) {
                         if (h > 0 && 4 * h >= n_units) break;
@@ -530,11 +548,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                                 fa += 4 * u;
                                 fb += 4 * C::kSfbBlocks * u;
                             }
-                            tcgen05_mma<C::KIND, C::CG>(one, d, da + u * kStepA, db + u * kStepB, id, fa, fb, kb > 0 || h > 0 || u > 0);
+                            tcgen05_mma<C::KIND, C::CG>(one, d, da + u * kStepA, db + u * kStepB, id, fa, fb, kb > k_first || h > 0 || u > 0);
                         }
                     }
                     tcgen05_commit<C::CG>(one, bar(&empty_bar[now]));
-                    if (kb + 1 == k_stages) tcgen05_commit<C::CG>(one, bar(&acc_full[a]));
+                    if (kb + 1 == k_last) tcgen05_commit<C::CG>(one, bar(&acc_full[a]));
                     ready = __any_sync(kFullMask, seen);
                 }
             }
@@ -553,7 +571,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 using Regs = decltype(regs_tag);
                 Regs r[2];
                 ScaleWalk<C> at;
-                at.begin(p, sched, unit);
+                at.begin(p, sched, unit, k_first, k_end);
                 at.advance(p, sched, units, (warp - 2) >> 1);
                 auto load = [&](Regs& regs) {
                     const GemmTile& tile = at.tile;
@@ -629,7 +647,16 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             for (uint32_t c = rw / 4 * 32; c < tile.jn; c += 8 * C::kResultWarps) {
                 const uint32_t n = min(32u, tile.jn - c);
                 uint32_t v[32];
-                if (C::WGRAD && p.out_f32) {
+                if constexpr (C::SPLIT) {
+                    tmem_load32(taddr + c, v);
+                    tmem_load_wait();
+                    // the owner of a column i keeps sums as [part][row j][its columns]
+                    const uint32_t own = 128 / p.split, i = quarter * 32 + lane;
+                    const uint32_t to = map_to_rank(partial + ((part * C::NMAX + c) * own + i % own) * 4, i / own);
+#pragma unroll
+                    for (uint32_t q = 0; q < 32; ++q)
+                        if (q < n) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + q * own * 4), "r"(v[q]) : "memory");
+                } else if (C::WGRAD && p.out_f32) {
                     store_f32<C>(p, tile, v, have, taddr + c, iw, c, n, lane);
                 } else {
                     store_bf16<C>(p, tile, v, have, taddr + c, iw, c, n, alpha, stage_mem + (turn & 1u) * 2048u, lane);
@@ -661,12 +688,30 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     __syncwarp();
     tcgen05_fence_before();
     __syncthreads();
-    if constexpr (C::CG == 2) cluster_sync();
+    if constexpr (C::CG == 2 || C::SPLIT) cluster_sync();
     if (warp == 1) {
         tcgen05_fence_after();
         tmem_dealloc<C::CG>(tmem, C::kCols);
     }
     if constexpr (C::CG == 2) cluster_sync();
+    if constexpr (C::SPLIT) {
+        if (unit < sched.total) {
+            const GemmTile tile = sched.tile(p, unit);
+            const float alpha = p.alpha == nullptr ? 1.0f : __ldg(p.alpha + static_cast<int64_t>(tile.e) * p.alpha_stride);
+            const uint32_t own = 128 / p.split;
+            for (uint32_t q = threadIdx.x; q < tile.jn * own; q += C::kThreads) {
+                const uint32_t j = q / own, i = tile.i0 + part * own + q % own;
+                float sum = 0.0f;
+                for (uint32_t from = 0; from < p.split; ++from) {
+                    float x;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(partial + ((from * C::NMAX + j) * own + q % own) * 4));
+                    sum = __fadd_rn(sum, x);
+                }
+                if (i < p.i_size)
+                    static_cast<__nv_bfloat16*>(p.out)[static_cast<int64_t>(tile.j0 + j) * p.out_stride + i] = __float2bfloat16_rn(__fmul_rn(sum, alpha));
+            }
+        }
+    }
 }
 
 }  // namespace tkq
