@@ -75,6 +75,8 @@ struct GemmConfig {
     static constexpr uint32_t kSfbBlocks = (NMAX + 127) / 128;
     static constexpr uint32_t kSfaBytes = 512 * kWords, kSfbBytes = 512 * kWords * kSfbBlocks;
     static constexpr uint32_t kStageBytes = kSub * (kABytes + kBBytes + kSfaBytes + kSfbBytes);
+    // Scale loaders: one warp per block of 128 rows (of A, and one or two of B), in sets that take stages in turn
+    static constexpr uint32_t kScaleBlocks = SCALED ? 1 + (NMAX + 127) / 128 : 1, kScaleSets = SCALED ? 6 / kScaleBlocks : 1;
     static constexpr uint32_t kLoaders = SCALED ? 6 : 2;  // warps between the two issuing ones and those that store results
     static constexpr uint32_t kFirstResultWarp = 2 + kLoaders, kResultWarps = 4;
     static constexpr uint32_t kThreads = 32 * (kFirstResultWarp + kResultWarps);
@@ -93,9 +95,9 @@ struct GemmConfig {
     static_assert(!SPLIT || (CG == 1 && !WGRAD), "the cluster of a split product is one along K");
     static_assert(!WGRAD || (A_MN && kBRows % 64 == 0 && kSub == 1), "weight gradient reads both operands along their rows");
     static_assert(kBBytes % 1024 == 0, "stage layout");
-    // A scale loader goes from stage `it` to `it` + 3.  It waits by parity, so the slot it comes to has to be at most one phase
-    // behind: MMA(it - kStages) is done by then, MMA(it + 3 - 2 kStages) has to be.
-    static_assert(kStages >= 3 && kStages >= kLoaders / 2, "a slot's parity would be ambiguous");
+    // A scale loader goes from stage `it` to `it` + kScaleSets.  It waits by parity, so the slot it comes to has to be at most one
+    // phase behind: MMA(it - kStages) is done by then, MMA(it + kScaleSets - 2 kStages) has to be.
+    static_assert(kStages >= 3 && kStages >= kScaleSets, "a slot's parity would be ambiguous");
 };
 
 struct GemmTile {
@@ -168,16 +170,16 @@ struct GemmSchedule {
     }
 };
 
-// Scale words of ROWBLK * 32 rows for one stage: lane l holds rows l, l + 32, ...
-template <class C, int ROWBLK>
+// Scale words of 128 rows for one stage: lane l holds rows l, l + 32, l + 64 and l + 96.
+template <class C>
 struct ScaleRegs {
     static constexpr uint32_t kStageWords = C::kSub * C::kWords;
-    uint32_t w[ROWBLK][kStageWords];
+    uint32_t w[4][kStageWords];
 
     __device__ __forceinline__ void load(const ScaleView& v, const uint32_t* group, uint32_t row0, uint32_t row_end, uint32_t stage, uint32_t lane) {
         const uint32_t word0 = v.k_shift ? stage >> 1 : stage * kStageWords;  // scales of 128 values: one word for two stages
 #pragma unroll
-        for (int c = 0; c < ROWBLK; ++c) {
+        for (int c = 0; c < 4; ++c) {
             const uint32_t row = row0 + lane + 32u * c;
             const uint32_t* at = group + static_cast<int64_t>(row >> v.row_shift) * v.row_stride + static_cast<int64_t>(word0) * v.k_stride;
             const bool valid = row < row_end;
@@ -198,24 +200,16 @@ struct ScaleRegs {
         }
     }
 
-    // The tensor core copies 512-byte blocks of 128 rows: row r at (r % 32) * 16 + (r / 32) * 4.
-    __device__ __forceinline__ void store(uint32_t smem, uint32_t lane) const {
-        constexpr int kBlocks = (ROWBLK + 3) / 4;
+    // The tensor core copies 512-byte blocks of 128 rows, row r at (r % 32) * 16 + (r / 32) * 4; `pitch` between words.
+    __device__ __forceinline__ void store(uint32_t smem, uint32_t pitch, uint32_t lane) const {
 #pragma unroll
         for (uint32_t k = 0; k < kStageWords; ++k)
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                uint32_t q[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) q[i] = 4 * b + i < ROWBLK ? w[4 * b + i < ROWBLK ? 4 * b + i : 0][k] : 0u;
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem + (k * kBlocks + b) * 512u + lane * 16u), "r"(q[0]), "r"(q[1]),
-                             "r"(q[2]), "r"(q[3])
-                             : "memory");
-            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem + k * pitch + lane * 16u), "r"(w[0][k]), "r"(w[1][k]), "r"(w[2][k]), "r"(w[3][k])
+                         : "memory");
     }
 };
 
-// A scale loader's place: stage `stage` of tile `tile`, the block's stage number `it`.
+// A scale loader's place: stage `stage` of tile `tile`.
 template <class C>
 struct ScaleWalk {
     GemmTile tile;
@@ -228,13 +222,11 @@ struct ScaleWalk {
         t = unit;
         first = stage = k_first;
         last = k_end;
-        it = 0;
         valid = t < sched.total;
         if (valid) tile = sched.tile(p, t);
     }
     __device__ __forceinline__ void advance(const GemmParams& p, const GemmSchedule<C>& sched, uint32_t units, uint32_t stages) {
         stage += stages;
-        it += stages;
         while (valid && stage >= last) {
             stage -= last - first;
             t += units;
@@ -394,7 +386,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             abort_flag = 0;
             for (uint32_t s = 0; s < C::kStages; ++s) {
                 // scale loaders of every CTA arrive beside the TMA bytes; the weight gradient signals through ready_bar
-                mbar_init(&full_bar[s], 1 + (C::SCALED ? 2 * C::CG : 0));
+                mbar_init(&full_bar[s], 1 + (C::SCALED ? C::kScaleBlocks * C::CG : 0));
                 mbar_init(&empty_bar[s], 1);
                 mbar_init(&ready_bar[s], C::CG);
             }
@@ -563,40 +555,43 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         }
     } else if (warp < C::kFirstResultWarp) {
         if constexpr (C::SCALED) {
-            // ---- scale factors: even warps those of A, odd ones those of B.  Three warps per operand take stages in turn, each with
-            // the loads of its next stage in flight: the words come from L2 while TMA loads keep its ports busy, and take about
-            // a microsecond.  (8192 x 4096 x 7168 MXFP4 136 us with one warp per operand and loads two blocks ahead, 105 us
-            // without any loads.) ----
-            auto run = [&](auto regs_tag, const ScaleView& v, uint32_t smem_off, bool is_a) {
-                using Regs = decltype(regs_tag);
-                Regs r[2];
-                ScaleWalk<C> at;
-                at.begin(p, sched, unit, k_first, k_end);
-                at.advance(p, sched, units, (warp - 2) >> 1);
-                auto load = [&](Regs& regs) {
-                    const GemmTile& tile = at.tile;
-                    regs.load(v, v.base + (is_a ? static_cast<int64_t>(tile.e) * v.group_stride : 0), is_a ? tile.i0 + rank * 128u : tile.j0,
-                              is_a ? p.i_size : tile.j0 + tile.jn, at.stage, lane);
-                };
-                if (at.valid) load(r[0]);
-                while (at.valid) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (!at.valid) break;
-                        const uint32_t it = at.it, s = it % C::kStages;
-                        at.advance(p, sched, units, C::kLoaders / 2);
-                        if (at.valid) load(r[h ^ 1]);
-                        const bool ok = wait(bar(&empty_bar[s]), ((it / C::kStages) & 1u) ^ 1u);
-                        if (!__all_sync(kFullMask, ok)) return;
-                        r[h].store(sf_base + s * (C::kSub * (C::kSfaBytes + C::kSfbBytes)) + smem_off, lane);
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(leader_bar(&full_bar[s]));
-                    }
-                }
+            // ---- scale factors.  A warp keeps the words of its next two stages on their way: they come from L2 while TMA loads
+            // keep its ports busy, and take about a microsecond.  (8192 x 4096 x 7168 in MXFP4 took 136 us with one warp per
+            // operand and loads two blocks ahead, NVFP4 143 us with loads one stage ahead and 126 us so.) ----
+            const uint32_t block = (warp - 2) % C::kScaleBlocks, set = (warp - 2) / C::kScaleBlocks;
+            const bool is_a = block == 0;
+            const ScaleView& v = is_a ? p.sfa : p.sfb;
+            const uint32_t to = sf_base + (is_a ? 0 : C::kSub * C::kSfaBytes + (block - 1) * 512u), pitch = is_a ? 512u : C::kSfbBlocks * 512u;
+            ScaleRegs<C> r[3];
+            ScaleWalk<C> ahead;  // the stage to load next; the stages to pass on follow two behind
+            ahead.begin(p, sched, unit, k_first, k_end);
+            ahead.advance(p, sched, units, set);
+            auto load = [&](ScaleRegs<C>& regs) {
+                const GemmTile& tile = ahead.tile;
+                regs.load(v, v.base + (is_a ? static_cast<int64_t>(tile.e) * v.group_stride : 0), is_a ? tile.i0 + rank * 128u : tile.j0 + (block - 1) * 128u,
+                          is_a ? p.i_size : tile.j0 + tile.jn, ahead.stage, lane);
+                ahead.advance(p, sched, units, C::kScaleSets);
             };
-            if ((warp & 1u) == 0) run(ScaleRegs<C, 4>{}, p.sfa, 0, true);
-            else run(ScaleRegs<C, (C::NMAX + 31) / 32>{}, p.sfb, C::kSub * C::kSfaBytes, false);
+            uint32_t it = set, loaded = 0;
+            if (ahead.valid) load(r[0]), ++loaded;
+            if (ahead.valid) load(r[1]), ++loaded;
+            bool ok = true;
+            while (ok && loaded > 0) {
+#pragma unroll
+                for (int h = 0; h < 3; ++h) {
+                    if (loaded == 0) break;
+                    if (ahead.valid) load(r[(h + 2) % 3]), ++loaded;
+                    const uint32_t s = it % C::kStages;
+                    ok = __all_sync(kFullMask, wait(bar(&empty_bar[s]), ((it / C::kStages) & 1u) ^ 1u));
+                    if (!ok) break;
+                    r[h].store(to + s * (C::kSub * (C::kSfaBytes + C::kSfbBytes)), pitch, lane);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(leader_bar(&full_bar[s]));
+                    it += C::kScaleSets;
+                    --loaded;
+                }
+            }
         } else if constexpr (C::WGRAD) {
             // ---- rows behind the group's end: the last stage's tail belongs to another group (or to nobody) and is cleared in
             // both operands, so that not even an infinity there can reach the sum ----
