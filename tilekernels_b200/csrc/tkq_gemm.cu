@@ -49,9 +49,11 @@ static bool fix_strides(Operand& o) {
 
 template <class C>
 static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const char* what, cudaStream_t stream) {
-    alignas(64) CUtensorMap map_a, map_b;
+    alignas(64) CUtensorMap map_a;
+    alignas(64) GemmMapsB maps_b{};
     if (int rc = encode(&map_a, a, C::A_MN ? 64 : C::kElems, C::A_MN ? 64 : 128)) return rc;
-    if (int rc = encode(&map_b, b, C::WGRAD ? 64 : C::kElems, C::WGRAD ? 64 : C::kBRows)) return rc;
+    for (uint32_t i = 0; i < C::kBoxes; ++i)
+        if (int rc = encode(&maps_b.box[i], b, C::WGRAD ? 64 : C::kElems, C::WGRAD ? 64 : C::kBRows >> i)) return rc;
     p.wide_out = p.i_size % 8 == 0 && p.out_stride % 8 == 0 && p.out_group_stride % 8 == 0 && aligned16(p.out);
     p.i_tiles = (p.i_size + 128 * C::CG - 1) / (128 * C::CG);
     const int64_t j_tiles = C::WGRAD ? int64_t{p.groups} * ((p.j_size + C::NMAX - 1) / C::NMAX) : int64_t{p.rows} / C::NMAX + p.groups;
@@ -73,7 +75,7 @@ static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const c
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = cluster > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, map_a, map_b, p);
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, map_a, maps_b, p);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return set_error(static_cast<int>(e), cudaGetErrorString(e));

@@ -88,6 +88,7 @@ struct GemmConfig {
     static constexpr uint32_t kSfBase = 2 * NMAX;
     static constexpr uint32_t kColsNeeded = 2 * NMAX + kSub * kSfCols;
     static constexpr uint32_t kCols = kColsNeeded <= 64 ? 64 : kColsNeeded <= 128 ? 128 : kColsNeeded <= 256 ? 256 : 512;
+    static constexpr uint32_t kBoxes = NMAX >= 96 && !WGRAD ? 3 : 1;
     static constexpr uint32_t kElems = KIND == kKindBf16 ? 64 : 128;  // tensor-map elements of a 128-byte row
     static constexpr uint32_t kNStep = CG == 2 ? 32 : 16;
     static_assert(kColsNeeded <= 512, "tensor memory");
@@ -98,6 +99,13 @@ struct GemmConfig {
     // A scale loader goes from stage `it` to `it` + kScaleSets.  It waits by parity, so the slot it comes to has to be at most one
     // phase behind: MMA(it - kStages) is done by then, MMA(it + kScaleSets - 2 kStages) has to be.
     static_assert(kStages >= 3 && kStages >= kScaleSets, "a slot's parity would be ambiguous");
+};
+
+// A tile's rows of B come in one box.  The last tile of a group often has few rows, and loads, which bound the products of
+// 256 x N tiles as much as the tensor core does, then take a box of a half or a quarter (16 experts of skewed sizes, bf16:
+// MEASURE).  Several small boxes instead of a large one are slower (312 -> 360 us on 8192 x 4096 x 7168).
+struct GemmMapsB {
+    CUtensorMap box[3];
 };
 
 struct GemmTile {
@@ -119,13 +127,6 @@ struct GemmWait {
         return false;
     }
 };
-
-// Rows of a group are dealt to ceil(rows / NMAX) tiles of about equal size, a multiple of the instruction's N step.
-template <class C>
-__device__ __forceinline__ uint32_t rows_per_tile(uint32_t rows) {
-    const uint32_t t = (rows + C::NMAX - 1) / C::NMAX;
-    return t == 0 ? C::kNStep : ((rows + t - 1) / t + C::kNStep - 1) / C::kNStep * C::kNStep;
-}
 
 template <class C>
 struct GemmSchedule {
@@ -151,7 +152,7 @@ struct GemmSchedule {
             }
             r.e = lo;
             local = t - prefix[lo];
-            per = rows_per_tile<C>(rows[lo]);
+            per = C::NMAX;
             j_tiles = (rows[lo] + per - 1) / per;
         }
         // bands of eight tiles along j: the tiles in flight share few rows of either operand, which stay in L2
@@ -294,7 +295,7 @@ __device__ __forceinline__ void store_bf16(const GemmParams& p, const GemmTile& 
 
 // fp32 results of the weight gradient: a warp's 32 lanes hold 32 neighbouring columns, 128 bytes of a row, so every store
 // is a whole line as it is.  (Shared memory is what the products are short of: staged rows and TMA stores took 600 us where
-// these take MEASURE, 16 experts, 8192 rows, 4096 x 7168.)  An accumulating call adds in L2, each element once.
+// these take 540, 16 experts, 8192 rows, 4096 x 7168.)  An accumulating call adds in L2, each element once.
 template <class C>
 __device__ __forceinline__ void store_f32(const GemmParams& p, const GemmTile& tile, uint32_t (&v)[32], bool have, uint32_t taddr, uint32_t iw,
                                           uint32_t c, uint32_t n, uint32_t lane) {
@@ -327,7 +328,7 @@ __device__ __forceinline__ void store_f32(const GemmParams& p, const GemmTile& t
 
 template <class C>
 __global__ void __launch_bounds__(C::kThreads, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmParams p) {
+    gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ GemmMapsB maps_b, const GemmParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full_bar[C::kStages], empty_bar[C::kStages], ready_bar[C::kStages], acc_full[2], acc_empty[2], drain_bar;
     __shared__ uint32_t tmem_slot;
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     if (warp == 0) {
         if (lane == 0) {
             prefetch_tensor_map(&map_a);
-            prefetch_tensor_map(&map_b);
+            prefetch_tensor_map(&maps_b.box[0]);
         }
         // group table: start and rows clamped to the tensor, tiles before each group
         uint32_t before = 0;
@@ -366,10 +367,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                     s = min(max(static_cast<int64_t>(p.start[e]), int64_t{0}), static_cast<int64_t>(p.rows));
                     t = min(max(static_cast<int64_t>(p.end[e]), s), static_cast<int64_t>(p.rows));
                 }
-                const uint32_t rows = static_cast<uint32_t>(t - s), per = rows_per_tile<C>(rows);
+                const uint32_t rows = static_cast<uint32_t>(t - s);
                 s_start[e] = static_cast<uint32_t>(s);
                 s_rows[e] = rows;
-                tiles = (rows + per - 1) / per * p.i_tiles;
+                tiles = (rows + C::NMAX - 1) / C::NMAX * p.i_tiles;
             }
             uint32_t sum = tiles;
 #pragma unroll
@@ -425,6 +426,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             const int32_t i0 = static_cast<int32_t>(tile.i0 + rank * 128u);
             const int32_t j0 = static_cast<int32_t>(tile.j0 + (C::CG == 2 ? rank * (tile.n_mma / 2) : 0));
             const uint32_t k_last = C::WGRAD ? tile.k_stages : k_end;
+            const uint32_t small = C::kBoxes == 1 ? 0 : 4 * tile.n_mma <= C::NMAX ? 2 : 2 * tile.n_mma <= C::NMAX ? 1 : 0;
+            const CUtensorMap* map_b = &maps_b.box[small];
             for (uint32_t kb = k_first; kb < k_last; ++kb) {
                 ok = __any_sync(kFullMask, one && wait(bar(&empty_bar[s]), phase));
                 if (!ok) break;
@@ -433,7 +436,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 const uint32_t full = C::WGRAD ? bar(&full_bar[s]) : leader_bar(&full_bar[s]);
                 if (one) {
                     if (C::WGRAD) mbar_arrive_expect_tx(&full_bar[s], C::kABytes + C::kBBytes);
-                    else if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], C::CG * C::kSub * (C::kABytes + C::kBBytes));
+                    else if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], C::CG * C::kSub * (C::kABytes + (C::kBBytes >> small)));
 #pragma unroll
                     for (uint32_t u = 0; u < C::kSub; ++u) {
                         const int32_t ku = k + static_cast<int32_t>(u * C::kElems);
@@ -447,10 +450,9 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                         if constexpr (C::WGRAD) {
 #pragma unroll
                             for (uint32_t q = 0; q < C::kBRows / 64; ++q)
-                                tma_load_3d<C::CG>(b + q * 8192, &map_b, j0 + static_cast<int32_t>(64 * q), ku, 0, full);
+                                tma_load_3d<C::CG>(b + q * 8192, map_b, j0 + static_cast<int32_t>(64 * q), ku, 0, full);
                         } else {
-                            // (one box: the same rows in boxes of 32 took bf16 products from 312 to 360 us)
-                            tma_load_3d<C::CG>(b + u * C::kBBytes, &map_b, ku, j0, 0, full);
+                            tma_load_3d<C::CG>(b + u * C::kBBytes, map_b, ku, j0, 0, full);
                         }
                     }
                 }
