@@ -70,6 +70,25 @@ def test_few_tiles_and_a_long_k(cuda_device, form, m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('form', FORMS, ids=_id)
+def test_many_waves(cuda_device, form):
+    """Several tiles per block, whose scales differ from block to block along k: every sum against 64 bits, on the device."""
+    from tilekernels_b200 import quant
+    fmt, ab, bb = form
+    m, n, k = 3000, 2600, 2048
+    a, b = _matrices(m, n, k, cuda_device)
+    (qa, va, ta), (qb, vb, tb) = quantize(a, fmt, ab), quantize(b, fmt, bb)
+    alpha = ta * tb if fmt == 'nvfp4' else torch.ones(1, device=cuda_device)
+    va, vb = va.to(cuda_device) * alpha.double(), vb.to(cuda_device)
+    want, magnitudes = va @ vb.T, va.abs() @ vb.abs().T
+    bound = k * 2.0 ** -23 * magnitudes
+    bound += 2.0 ** -8 * (want.abs() + bound)
+    for _ in range(3):
+        got = quant.block_scaled_gemm(qa, qb, ab, bb, alpha=alpha)
+        assert ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('m', (1, 300))
 def test_alpha_out_and_strides(cuda_device, m):
     from tilekernels_b200 import quant

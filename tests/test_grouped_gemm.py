@@ -211,6 +211,24 @@ def test_many_experts(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('form', (('e4m3', (1, 128), (128, 128)), ('e2m1', (1, 32), (1, 32)), ('nvfp4', (1, 16), (1, 16))), ids=lambda f: f[0])
+def test_many_experts_with_many_rows(cuda_device, form):
+    """More groups than a tile variant with large shared-memory needs has a table for."""
+    from tilekernels_b200 import moe
+    fmt, xb, wb = form
+    experts, n, k = 130, 128, 128
+    sizes = [(37 * i) % 140 for i in range(experts)]
+    x, start, end, member = _rows(sizes, k, cuda_device)
+    x[~member.to(cuda_device)] = 0
+    xq, xv, xt = quantize(x, fmt, xb)
+    w = torch.randn((experts * n, k), generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda_device)
+    wq, wv, wt = quantize(w, fmt, wb)
+    alpha = xt * wt if fmt == 'nvfp4' else None
+    got = moe.grouped_gemm(xq, (wq[0].view(experts, n, -1), wq[1]), int32(start, cuda_device), int32(end, cuda_device), xb, wb, alpha=alpha)
+    _check_groups(got, xv, wv.view(experts, n, k), start, end, scale=None if alpha is None else [alpha.double().item()] * experts)
+
+
+@pytest.mark.gpu
 def test_no_rows(cuda_device):
     from tilekernels_b200 import moe
     w = torch.ones((2, 16, 64), dtype=torch.bfloat16, device=cuda_device)

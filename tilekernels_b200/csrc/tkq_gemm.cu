@@ -60,6 +60,7 @@ static int launch_gemm(const Operand& a, const Operand& b, GemmParams p, const c
     if (j_tiles * p.i_tiles >= (int64_t{1} << 31)) return set_error(TKQ_E_UNSUPPORTED, "matrix product: more than 2^31 tiles");
     // CTAs of a cluster: a pair on one tile, or those that share a tile along K
     const int cluster = C::SPLIT ? static_cast<int>(p.split) : C::CG;
+    if (p.groups > C::kGroups) return set_error(TKQ_E_UNSUPPORTED, "matrix product: more groups than the tile variant's table holds");
     const int64_t units = std::min<int64_t>(j_tiles * p.i_tiles, device_sm_count() / cluster);
     const int smem = static_cast<int>(1024 + C::kStages * C::kStageBytes + C::kStagingBytes + C::kPartialBytes + 4 * (3 * p.groups + 1));
     auto kernel = gemm_kernel<C>;
@@ -119,6 +120,9 @@ static int launch_rows(const Operand& a, const Operand& b, const GemmParams& p, 
     if (mean <= 128 && launch_split<KIND, 64, A_MN>(a, b, p, what, stream, &rc)) return rc;
     if (mean <= 48 || row_tiles(p, NMID) * ((p.i_size + 127) / 128) <= device_sm_count())
         return launch_gemm<GemmConfig<KIND, 1, NMID, false, A_MN>>(a, b, p, what, stream);
+    // NVFP4: 224 rows a tile where the group table fits beside them (8192 x 4096 x 7168: 121 us with 192, 111 us with 224)
+    if constexpr (KIND == kKindNvf4)
+        if (p.groups > GemmConfig<KIND, 2, NLARGE, false, A_MN>::kGroups) return launch_gemm<GemmConfig<KIND, 2, 192, false, A_MN>>(a, b, p, what, stream);
     return launch_gemm<GemmConfig<KIND, 2, NLARGE, false, A_MN>>(a, b, p, what, stream);
 }
 
@@ -196,7 +200,7 @@ extern "C" int tkq_block_scaled_gemm(const void* x, int64_t x_row_stride, const 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (fp8) return launch_rows<kKindMxf8, 128, 224, false>(a, b, p, "block_scaled_gemm", s);
     if (!nv) return launch_rows<kKindMxf4, 128, 224, false>(a, b, p, "block_scaled_gemm", s);
-    return launch_rows<kKindNvf4, 96, 192, false>(a, b, p, "block_scaled_gemm", s);
+    return launch_rows<kKindNvf4, 96, 224, false>(a, b, p, "block_scaled_gemm", s);
 }
 
 extern "C" int tkq_grouped_gemm(const void* x, int64_t x_row_stride, const void* w, int64_t w_expert_stride, int64_t w_row_stride, int transpose_w,

@@ -31,7 +31,7 @@
 namespace tkq {
 
 constexpr int kMaxGroups = 1024;
-constexpr uint32_t kGemmSmemBudget = 232448 - 1024 /* alignment */ - 512 /* barriers */ - 12 * (kMaxGroups + 1);
+constexpr uint32_t kGemmSmemBudget = 232448 - 1024 /* alignment */ - 512 /* barriers */;
 
 // Scale factors of one operand: the 32-bit word with the scales of row r and K-words k of group e is
 // base[e * group_stride + (r >> row_shift) * row_stride + k * k_stride].
@@ -82,11 +82,15 @@ struct GemmConfig {
     static constexpr uint32_t kThreads = 32 * (kFirstResultWarp + kResultWarps);
     static constexpr uint32_t kStagingPerWarp = SCALED ? 2048 : 4096, kStagingBytes = kStagingPerWarp * kResultWarps;
     static constexpr uint32_t kPartialBytes = SPLIT ? NMAX * 128 * 4 : 0;
-    static constexpr uint32_t kFits = (kGemmSmemBudget - kStagingBytes - kPartialBytes) / kStageBytes;
+    // (NVFP4 with 224 rows: the scales leave room for three stages and a table of fewer groups)
+    static constexpr uint32_t kGroups = KIND == kKindNvf4 && NMAX > 192 ? 96 : kMaxGroups;
+    static constexpr uint32_t kFits = (kGemmSmemBudget - kStagingBytes - kPartialBytes - 12 * (kGroups + 1)) / kStageBytes;
     static constexpr uint32_t kStages = kFits < 10 ? kFits : 10;
     static constexpr uint32_t kSfCols = 4 * kWords * (1 + kSfbBlocks);  // tensor-memory columns of one block's scales
     static constexpr uint32_t kSfBase = 2 * NMAX;
-    static constexpr uint32_t kColsNeeded = 2 * NMAX + kSub * kSfCols;
+    // two sets of scale columns that blocks take in turn, or one where two do not fit beside the accumulators
+    static constexpr uint32_t kSfSets = 2 * NMAX + kSub * kSfCols <= 512 ? kSub : 1;
+    static constexpr uint32_t kColsNeeded = 2 * NMAX + kSfSets * kSfCols;
     static constexpr uint32_t kCols = kColsNeeded <= 64 ? 64 : kColsNeeded <= 128 ? 128 : kColsNeeded <= 256 ? 256 : 512;
     static constexpr uint32_t kBoxes = NMAX >= 96 && !WGRAD ? 3 : 1;
     static constexpr uint32_t kElems = KIND == kKindBf16 ? 64 : 128;  // tensor-map elements of a 128-byte row
@@ -511,11 +515,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                     for (uint32_t h = 0; h < C::kSub; ++h) {
                         if (h > 0 && 4 * h >= n_units) break;
                         const uint64_t da = desc_a + (now * C::kSub + h) * (C::kABytes >> 4), db = desc_b + (now * C::kSub + h) * (C::kBBytes >> 4);
-                        const uint32_t sfa = tmem + C::kSfBase + h * C::kSfCols, sfb = sfa + 4 * C::kWords;
+                        const uint32_t sfa = tmem + C::kSfBase + h % C::kSfSets * C::kSfCols, sfb = sfa + 4 * C::kWords;
                         uint32_t id0 = idesc;
                         if constexpr (C::SCALED) {
-                            // The copies go over the scales of the block two before.  Copies and products of one thread run in the
-                            // order of their issue (they share a pipe), so nothing has to be waited for.
+                            // The copies go over the scales of an earlier block.  Copies and products of one thread run in the order of
+                            // their issue (they share a pipe), so nothing has to be waited for.
                             const uint64_t dfa = desc_sf + now * ((C::kSub * (C::kSfaBytes + C::kSfbBytes)) >> 4);
                             const uint64_t dfb = dfa + ((C::kSub * C::kSfaBytes) >> 4);
                             const uint32_t ha = C::KIND == kKindMxf8 && p.sfa.k_shift ? 0 : h, hb = C::KIND == kKindMxf8 && p.sfb.k_shift ? 0 : h;
