@@ -140,6 +140,23 @@ def test_wgrad(cuda_device, name, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('rows', (250, 1025, 9000))
+def test_wgrad_of_long_groups_keeps_its_precision(cuda_device, rows):
+    """The tensor core's sum goes on in registers every 256 rows.  A step of 16 rows cuts off at most one unit (2^-23 of the
+    sum of magnitudes) per term and once for the accumulator, so 256 rows are off by at most 272 units; every addition in
+    registers rounds by at most half a unit."""
+    from tilekernels_b200 import moe
+    n, k = 136, 264
+    gen = torch.Generator().manual_seed(rows)
+    g = (torch.rand((rows, n), generator=gen) + 0.5).to(torch.bfloat16).to(cuda_device)   # one sign: nothing averages out
+    x = (torch.rand((rows, k), generator=gen) + 0.5).to(torch.bfloat16).to(cuda_device)
+    got = moe.grouped_gemm_wgrad(g, x, int32([0], cuda_device), int32([rows], cuda_device))[0]
+    want = g.double().T @ x.double()
+    bound = (272 * 2.0 ** -23 + -(-rows // 256) * 2.0 ** -24) * want
+    assert ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences(cuda_device):
     """The product is linear in either operand, and with small integers every sum is exact, so differences of the forward
     product have to equal the gradients to the last bit."""

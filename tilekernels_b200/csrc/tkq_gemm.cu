@@ -261,8 +261,8 @@ extern "C" int tkq_grouped_gemm_wgrad(const void* grad, int64_t grad_row_stride,
     p.rows = static_cast<uint32_t>(num_rows);
     p.i_size = static_cast<uint32_t>(k);
     p.j_size = static_cast<uint32_t>(n);
-    p.out_f32 = out_dtype == TKQ_DT_FP32;
     p.accumulate = (flags & TKQ_ACCUMULATE) ? 1 : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (out_dtype == TKQ_DT_FP32) return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true, false, true>>(a, b, p, "grouped_gemm_wgrad", s);
     return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true>>(a, b, p, "grouped_gemm_wgrad", s);
 }

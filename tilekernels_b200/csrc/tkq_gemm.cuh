@@ -58,14 +58,16 @@ struct GemmParams {
     uint32_t k_stages, last_units;  // forward: stages along K, matrix instructions of the last one
     uint32_t alpha_stride;
     uint32_t split;  // CTAs of a cluster that share a tile along K
-    uint32_t out_f32, accumulate, zero_gaps;
+    uint32_t accumulate, zero_gaps;
     uint32_t wide_out;  // rows of out on 16-byte boundaries and i_size a multiple of 8
 };
 
-template <int KIND_, int CG_, int NMAX_, bool WGRAD_, bool A_MN_, bool SPLIT_ = false>
+template <int KIND_, int CG_, int NMAX_, bool WGRAD_, bool A_MN_, bool SPLIT_ = false, bool F32_ = false>
 struct GemmConfig {
     static constexpr int KIND = KIND_, CG = CG_, NMAX = NMAX_;
-    static constexpr bool WGRAD = WGRAD_, A_MN = A_MN_, SCALED = KIND_ != kKindBf16, SPLIT = SPLIT_;
+    static constexpr bool WGRAD = WGRAD_, A_MN = A_MN_, SCALED = KIND_ != kKindBf16, SPLIT = SPLIT_, F32 = F32_;
+    // fp32 results: stages whose products the tensor core adds up before the sum goes on in registers (see add_f32)
+    static constexpr uint32_t kChunk = F32 ? 4 : 1u << 30;
     // A stage holds kSub blocks of 128 bytes along K.  Waiting for a stage and handing it back costs the issuing warp some
     // 200 cycles: two thirds of a block's products in 4 or 8 bits (448 cycles at N = 224), which therefore come in pairs
     static constexpr uint32_t kSub = SCALED ? 2 : 1;
@@ -78,9 +80,9 @@ struct GemmConfig {
     // Scale loaders: one warp per block of 128 rows (of A, and one or two of B), in sets that take stages in turn
     static constexpr uint32_t kScaleBlocks = SCALED ? 1 + (NMAX + 127) / 128 : 1, kScaleSets = SCALED ? 6 / kScaleBlocks : 1;
     static constexpr uint32_t kLoaders = SCALED ? 6 : 2;  // warps between the two issuing ones and those that store results
-    static constexpr uint32_t kFirstResultWarp = 2 + kLoaders, kResultWarps = 4;
+    static constexpr uint32_t kFirstResultWarp = 2 + kLoaders, kResultWarps = F32 ? 8 : 4;
     static constexpr uint32_t kThreads = 32 * (kFirstResultWarp + kResultWarps);
-    static constexpr uint32_t kStagingPerWarp = SCALED ? 2048 : 4096, kStagingBytes = kStagingPerWarp * kResultWarps;
+    static constexpr uint32_t kStagingPerWarp = F32 ? 0 : SCALED ? 2048 : 4096, kStagingBytes = kStagingPerWarp * kResultWarps;
     static constexpr uint32_t kPartialBytes = SPLIT ? NMAX * 128 * 4 : 0;
     // (NVFP4 with 224 rows: the scales leave room for three stages and a table of fewer groups)
     static constexpr uint32_t kGroups = KIND == kKindNvf4 && NMAX > 192 ? 96 : kMaxGroups;
@@ -297,33 +299,40 @@ __device__ __forceinline__ void store_bf16(const GemmParams& p, const GemmTile& 
     }
 }
 
-// fp32 results of the weight gradient: a warp's 32 lanes hold 32 neighbouring columns, 128 bytes of a row, so every store
-// is a whole line as it is.  (Shared memory is what the products are short of: staged rows and TMA stores took 600 us where
-// these take 540, 16 experts, 8192 rows, 4096 x 7168.)  An accumulating call adds in L2, each element once.
-template <class C>
-__device__ __forceinline__ void store_f32(const GemmParams& p, const GemmTile& tile, uint32_t (&v)[32], bool have, uint32_t taddr, uint32_t iw,
-                                          uint32_t c, uint32_t n, uint32_t lane) {
-    if (have) {
-        tmem_load32(taddr, v);
-        tmem_load_wait();
-    } else {
+// fp32 results of the weight gradient.  The tensor core cuts off what an addition to its accumulator shifts out instead of
+// rounding, so a long sum drifts towards zero by about 2.3e-8 of itself per step of 16 rows (groups of some 900 rows: 1.3e-6
+// off).  Every 16 steps its sum is therefore added to one in registers, with rounding: eight warps hold 128 columns of the
+// tile each, and the accumulators take turns, so that this goes on beside the products (16 experts, 8192 rows, 4096 x 7168:
+// 2.4e-7 off and 560 us; 4.8e-7 and 552 us with 32 steps; 1.3e-6 and 540 us without).
+__device__ __forceinline__ void add_f32(float (&sum)[128], uint32_t taddr, uint32_t columns) {
 #pragma unroll
-        for (int q = 0; q < 32; ++q) v[q] = 0;
+    for (uint32_t g = 0; g < 8; ++g) {
+        if (16 * g < columns) {
+            uint32_t v[16];
+            tmem_load16(taddr + 16 * g, v);
+            tmem_load_wait();
+#pragma unroll
+            for (uint32_t q = 0; q < 16; ++q) sum[16 * g + q] = __fadd_rn(sum[16 * g + q], __uint_as_float(v[q]));
+        }
     }
-    float* o = static_cast<float*>(p.out) + static_cast<int64_t>(tile.e) * p.out_group_stride + static_cast<int64_t>(tile.j0 + c) * p.out_stride + iw + lane;
-    if (iw + lane >= p.i_size) return;
-    if (n == 32 && !p.accumulate) {
+}
+
+// A warp's 32 lanes hold 32 neighbouring columns, 128 bytes of a row, so every store is a whole line as it is.  (Shared memory
+// is what the products are short of: staged rows and TMA stores took 600 us where these took 540, 16 experts, 8192 rows,
+// 4096 x 7168.)  An accumulating call adds in L2, each element once.
+__device__ __forceinline__ void store_f32(const GemmParams& p, const float (&sum)[128], float* o, uint32_t rows) {
+    if (rows >= 128 && !p.accumulate) {
 #pragma unroll
-        for (uint32_t q = 0; q < 32; ++q) {
-            asm volatile("st.global.L1::no_allocate.b32 [%0], %1;" ::"l"(o), "r"(v[q]) : "memory");
+        for (uint32_t q = 0; q < 128; ++q) {
+            asm volatile("st.global.L1::no_allocate.f32 [%0], %1;" ::"l"(o), "f"(sum[q]) : "memory");
             o += p.out_stride;
         }
     } else {
 #pragma unroll
-        for (uint32_t q = 0; q < 32; ++q) {
-            if (q < n) {
-                if (p.accumulate) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(o), "f"(__uint_as_float(v[q])) : "memory");
-                else *o = __uint_as_float(v[q]);
+        for (uint32_t q = 0; q < 128; ++q) {
+            if (q < rows) {
+                if (p.accumulate) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(o), "f"(sum[q]) : "memory");
+                else *o = sum[q];
             }
             o += p.out_stride;
         }
@@ -492,16 +501,21 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 const GemmTile tile = sched.tile(p, t);
                 const uint32_t k_last = C::WGRAD ? tile.k_stages : k_end;
                 if (k_last == 0) continue;
-                const uint32_t a = acc_it & 1u;
-                ok = __any_sync(kFullMask, one && wait(bar(&acc_empty[a]), ((acc_it >> 1) & 1u) ^ 1u));
-                if (!ok) break;
-                ++acc_it;
-                tcgen05_fence_after();
-                const uint32_t d = tmem + a * C::NMAX;
+                uint32_t a = 0, d = 0;
                 uint32_t idesc;
                 if constexpr (C::SCALED) idesc = idesc_scaled(kM, tile.n_mma, C::KIND == kKindMxf8 ? 0 : 1, C::KIND != kKindNvf4);
                 else idesc = idesc_bf16(kM, tile.n_mma, C::A_MN, C::WGRAD);
                 for (uint32_t kb = k_first; kb < k_last; ++kb) {
+                    const bool opens = kb == k_first || (C::F32 && kb % C::kChunk == 0);
+                    const bool closes = kb + 1 == k_last || (C::F32 && (kb + 1) % C::kChunk == 0);
+                    if (opens) {
+                        a = acc_it & 1u;
+                        ok = __any_sync(kFullMask, one && wait(bar(&acc_empty[a]), ((acc_it >> 1) & 1u) ^ 1u));
+                        if (!ok) break;
+                        ++acc_it;
+                        tcgen05_fence_after();
+                        d = tmem + a * C::NMAX;
+                    }
                     if (!ready) ok = __any_sync(kFullMask, one && wait(bar(C::WGRAD ? &ready_bar[s] : &full_bar[s]), phase));
                     if (!ok) break;
                     tcgen05_fence_after();
@@ -546,11 +560,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                                 fa += 4 * u;
                                 fb += 4 * C::kSfbBlocks * u;
                             }
-                            tcgen05_mma<C::KIND, C::CG>(one, d, da + u * kStepA, db + u * kStepB, id, fa, fb, kb > k_first || h > 0 || u > 0);
+                            tcgen05_mma<C::KIND, C::CG>(one, d, da + u * kStepA, db + u * kStepB, id, fa, fb, !opens || h > 0 || u > 0);
                         }
                     }
                     tcgen05_commit<C::CG>(one, bar(&empty_bar[now]));
-                    if (kb + 1 == k_last) tcgen05_commit<C::CG>(one, bar(&acc_full[a]));
+                    if (closes) tcgen05_commit<C::CG>(one, bar(&acc_full[a]));
                     ready = __any_sync(kFullMask, seen);
                 }
             }
@@ -631,7 +645,33 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         const uint32_t quarter = warp & 3u, rw = warp - C::kFirstResultWarp;
         const uint32_t stage_mem = staging + rw * C::kStagingPerWarp;
         uint32_t acc_it = 0, turn = 0;
-        for (uint32_t t = unit; t < sched.total; t += units) {
+        if constexpr (C::F32) {
+            bool ok = true;
+            for (uint32_t t = unit; ok && t < sched.total; t += units) {
+                const GemmTile tile = sched.tile(p, t);
+                if (tile.k_stages == 0 && p.accumulate) continue;
+                const uint32_t c = rw / 4 * 128, columns = tile.jn > c ? tile.jn - c : 0;  // the warp's 128 columns of the tile
+                float sum[128];
+#pragma unroll
+                for (uint32_t q = 0; q < 128; ++q) sum[q] = 0.0f;
+                for (uint32_t kb = 0; kb < tile.k_stages; kb += C::kChunk) {
+                    const uint32_t a = acc_it & 1u;
+                    ok = __all_sync(kFullMask, wait(bar(&acc_full[a]), (acc_it >> 1) & 1u));
+                    if (!ok) break;
+                    ++acc_it;
+                    tcgen05_fence_after();
+                    add_f32(sum, tmem + a * C::NMAX + c + (quarter << 21), columns);
+                    tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(leader_bar(&acc_empty[a]));
+                }
+                const uint32_t i = tile.i0 + rank * 128u + quarter * 32u + lane;
+                if (ok && i < p.i_size)
+                    store_f32(p, sum, static_cast<float*>(p.out) + static_cast<int64_t>(tile.e) * p.out_group_stride +
+                                          static_cast<int64_t>(tile.j0 + c) * p.out_stride + i, columns);
+            }
+        }
+        for (uint32_t t = unit; !C::F32 && t < sched.total; t += units) {
             const GemmTile tile = sched.tile(p, t);
             const uint32_t a = acc_it & 1u;
             const bool have = tile.k_stages > 0;
@@ -657,8 +697,6 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 #pragma unroll
                     for (uint32_t q = 0; q < 32; ++q)
                         if (q < n) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + q * own * 4), "r"(v[q]) : "memory");
-                } else if (C::WGRAD && p.out_f32) {
-                    store_f32<C>(p, tile, v, have, taddr + c, iw, c, n, lane);
                 } else {
                     store_bf16<C>(p, tile, v, have, taddr + c, iw, c, n, alpha, stage_mem + (turn & 1u) * 2048u, lane);
                     if (C::kStagingPerWarp > 2048) ++turn;
