@@ -365,13 +365,26 @@ int tkq_cast_back_nvfp4(const void* x, const void* sf, const float* tensor_scale
  *   alpha            NULL or fp32, alpha[e * alpha_stride]
  *   out              bf16 [num_rows, out_row_stride]; rows of no group are left alone, or cleared with TKQ_ZERO_GAPS
  */
-int tkq_block_scaled_gemm(const void* x, int64_t x_row_stride, const void* x_sf, int64_t x_sf_row_stride, int64_t x_sf_k_stride,
-                          int x_block_m, int x_block_k, const void* w, int64_t w_expert_stride, int64_t w_row_stride,
-                          const void* w_sf, int64_t w_sf_expert_stride, int64_t w_sf_row_stride, int64_t w_sf_k_stride,
-                          int w_block_m, int w_block_k, int fmt, int sf_fmt, const int32_t* expert_start,
-                          const int32_t* expert_end, int64_t num_experts, int64_t num_rows, int64_t n, int64_t k,
-                          const float* alpha, int64_t alpha_stride, void* out, int64_t out_row_stride, unsigned flags,
-                          void* stream);
+typedef struct tkq_block_scaled_gemm_args { /* 8-byte fields only: it can be packed as an array of int64 */
+    const void* x;
+    int64_t x_row_stride;
+    const void* x_sf;
+    int64_t x_sf_row_stride, x_sf_k_stride, x_block_m, x_block_k;
+    const void* w;
+    int64_t w_expert_stride, w_row_stride;
+    const void* w_sf;
+    int64_t w_sf_expert_stride, w_sf_row_stride, w_sf_k_stride, w_block_m, w_block_k;
+    int64_t fmt, sf_fmt;
+    const int32_t* expert_start;
+    const int32_t* expert_end;
+    int64_t num_experts, num_rows, n, k;
+    const float* alpha;
+    int64_t alpha_stride;
+    void* out;
+    int64_t out_row_stride, flags;
+} tkq_block_scaled_gemm_args;
+
+int tkq_block_scaled_gemm(const tkq_block_scaled_gemm_args* args, void* stream);
 
 /*
  * bf16 products grouped by expert: out[r, i] = sum_k x[r, k] * w[e, i, k], or with transpose_w (the gradient of the rows)

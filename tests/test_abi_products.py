@@ -15,19 +15,20 @@ def lib():
 def test_argument_checks_of_the_products(lib):
     buf = (ctypes.c_char * 4096)()
     p16 = (ctypes.addressof(buf) + 15) // 16 * 16
+    from tilekernels_b200 import _lib
     scaled = lib.tkq_block_scaled_gemm
-    # (x, row stride, x_sf, sf row stride, sf k stride, block_m, block_k, w, expert stride, row stride, w_sf, sf expert, row, k
-    #  strides, block_m, block_k, fmt, sf_fmt, start, end, experts, rows, n, k, alpha, alpha stride, out, out stride, flags, stream)
-
-    def call(x=p16, xs=128, xbk=128, wbk=128, xbm=1, fmt=0, sf_fmt=0, experts=1, rows=4, n=8, k=128, start=None, end=None, out=p16, flags=0,
+    def call(x=p16, xs=128, xbk=128, wbk=128, xbm=1, fmt=0, sf_fmt=0, experts=1, rows=4, n=8, k=128, start=0, end=0, out=p16, flags=0,
              x_sf=p16):
-        return scaled(x, xs, x_sf, 1, 4, xbm, xbk, p16, 0, 128, p16, 0, 1, 8, 1, wbk, fmt, sf_fmt, start, end, experts, rows, n, k, None, 0, out,
-                      n, flags, None)
+        # x, row stride, x_sf, its row and k strides, block_m, block_k, w, expert and row strides, w_sf, its expert, row and k
+        # strides, block_m, block_k, fmt, sf_fmt, start, end, experts, rows, n, k, alpha, its stride, out, its stride, flags
+        return scaled(_lib.BLOCK_SCALED_GEMM_ARGS.pack(x, xs, x_sf, 1, 4, xbm, xbk, p16, 0, 128, p16, 0, 1, 8, 1, wbk, fmt, sf_fmt, start, end, experts,
+                                                       rows, n, k, 0, 0, out, n, flags), None)
 
+    assert scaled(None, None) == -1
     assert call(rows=0) == 0                                    # nothing to do
     assert call(rows=-1) == -1 and call(n=0) == -1 and call(k=0) == -1 and call(experts=0) == -1
     assert call(fmt=2) == -1 and call(sf_fmt=3) == -1
-    assert call(x=None) == -1 and call(out=None) == -1
+    assert call(x=0) == -1 and call(out=0) == -1
     assert call(start=p16) == -1 and call(experts=2) == -1      # bounds come in pairs, and groups need them
     assert call(experts=1025, start=p16, end=p16) == -2
     assert call(xbk=64) == -2 and call(xbm=16) == -2 and call(sf_fmt=1) == -2 and call(fmt=1) == -2

@@ -138,22 +138,22 @@ static int check_sizes(int64_t num_experts, int64_t num_rows, int64_t n, int64_t
 
 using namespace tkq;
 
-extern "C" int tkq_block_scaled_gemm(const void* x, int64_t x_row_stride, const void* x_sf, int64_t x_sf_row_stride, int64_t x_sf_k_stride,
-                                     int x_block_m, int x_block_k, const void* w, int64_t w_expert_stride, int64_t w_row_stride, const void* w_sf,
-                                     int64_t w_sf_expert_stride, int64_t w_sf_row_stride, int64_t w_sf_k_stride, int w_block_m, int w_block_k,
-                                     int fmt, int sf_fmt, const int32_t* expert_start, const int32_t* expert_end, int64_t num_experts,
-                                     int64_t num_rows, int64_t n, int64_t k, const float* alpha, int64_t alpha_stride, void* out,
-                                     int64_t out_row_stride, unsigned flags, void* stream) {
+extern "C" int tkq_block_scaled_gemm(const tkq_block_scaled_gemm_args* args, void* stream) {
+    static_assert(sizeof(tkq_block_scaled_gemm_args) == 29 * 8, "8-byte fields only");
+    if (args == nullptr) return set_error(TKQ_E_BAD_ARG, "block_scaled_gemm: null pointer");
+    const auto [x, x_row_stride, x_sf, x_sf_row_stride, x_sf_k_stride, x_block_m, x_block_k, w, w_expert_stride, w_row_stride, w_sf,
+                w_sf_expert_stride, w_sf_row_stride, w_sf_k_stride, w_block_m, w_block_k, fmt, sf_fmt, expert_start, expert_end, num_experts, num_rows,
+                n, k, alpha, alpha_stride, out, out_row_stride, flags] = *args;
     if (int rc = check_sizes(num_experts, num_rows, n, k)) return rc;
     if ((fmt != TKQ_FMT_E4M3 && fmt != TKQ_FMT_E2M1) || (sf_fmt != TKQ_SFMT_UE8M0 && sf_fmt != TKQ_SFMT_E4M3))
         return set_error(TKQ_E_BAD_ARG, "block_scaled_gemm: unknown format");
-    if (flags & ~static_cast<unsigned>(TKQ_ZERO_GAPS)) return set_error(TKQ_E_UNSUPPORTED, "block_scaled_gemm: only TKQ_ZERO_GAPS applies");
+    if (flags & ~int64_t{TKQ_ZERO_GAPS}) return set_error(TKQ_E_UNSUPPORTED, "block_scaled_gemm: only TKQ_ZERO_GAPS applies");
     if (num_rows == 0) return 0;
     if (x == nullptr || x_sf == nullptr || w == nullptr || w_sf == nullptr || out == nullptr || (expert_start == nullptr) != (expert_end == nullptr) ||
         (expert_start == nullptr && num_experts != 1))
         return set_error(TKQ_E_BAD_ARG, "block_scaled_gemm: null pointer");
     const bool fp8 = fmt == TKQ_FMT_E4M3, nv = sf_fmt == TKQ_SFMT_E4M3;
-    auto shift_of = [](int v) { return v == 1 ? 0 : v == 32 ? 5 : v == 128 ? 7 : -1; };
+    auto shift_of = [](int64_t v) { return v == 1 ? 0 : v == 32 ? 5 : v == 128 ? 7 : -1; };
     const int xs = shift_of(x_block_m), ws = shift_of(w_block_m);
     bool group_ok;
     if (fp8) group_ok = !nv && (x_block_k == 32 || x_block_k == 128) && (w_block_k == 32 || w_block_k == 128);
@@ -183,7 +183,7 @@ extern "C" int tkq_block_scaled_gemm(const void* x, int64_t x_row_stride, const 
     p.k_stages = static_cast<uint32_t>((row_bytes + 255) / 256);
     p.last_units = static_cast<uint32_t>((row_bytes - (int64_t{p.k_stages} - 1) * 256) / 32);
     p.zero_gaps = (flags & TKQ_ZERO_GAPS) ? 1 : 0;
-    auto view = [&](const void* sf, int64_t e, int64_t r, int64_t q, int shift, int block_k) {
+    auto view = [k = k](const void* sf, int64_t e, int64_t r, int64_t q, int shift, int64_t block_k) {
         ScaleView v{};
         v.base = static_cast<const uint32_t*>(sf);
         v.group_stride = e;

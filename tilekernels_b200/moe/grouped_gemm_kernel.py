@@ -6,7 +6,7 @@ import torch
 
 from .. import _lib
 from ..quant.block_scaled_gemm_kernel import ScaledOperand, check_out, launch_block_scaled_gemm
-from ..quant.common import DTYPE_TO_ENUM, current_stream_ptr, device_guard
+from ..quant.common import DTYPE_TO_ENUM, current_stream_ptr, device_guard, empty_matrix
 from ..quant.types import QuantTensor
 
 
@@ -69,7 +69,7 @@ def grouped_gemm(
     _check_groups(expert_start, expert_end, num_experts, like)
     device = like.device
     if out is None:
-        out = torch.empty((num_rows, n), dtype=torch.bfloat16, device=device)
+        out = empty_matrix(num_rows, n, torch.bfloat16, device)
     else:
         check_out(out, (num_rows, n), like)
     if quantized:

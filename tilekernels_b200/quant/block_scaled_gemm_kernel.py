@@ -5,7 +5,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .common import current_stream_ptr, device_guard
+from .common import current_stream_ptr, device_guard, empty_matrix
 from .types import QuantTensor
 
 
@@ -68,7 +68,7 @@ def launch_block_scaled_gemm(x: ScaledOperand, w: ScaledOperand, expert_start, e
     assert x.k > 0 and x.k == w.k, f'inner sizes differ: {x.k} and {w.k}'
     assert x.fmt == w.fmt and x.sf_fmt == w.sf_fmt, 'both operands must have the same format'
     assert x.data.get_device() == w.data.get_device()
-    alpha_ptr, alpha_stride = None, 0
+    alpha_ptr, alpha_stride = 0, 0
     if alpha is not None:
         assert alpha.dtype is torch.float32 and alpha.get_device() == x.data.get_device() and alpha.dim() <= 1
         assert alpha.numel() in (1, num_experts)
@@ -76,13 +76,14 @@ def launch_block_scaled_gemm(x: ScaledOperand, w: ScaledOperand, expert_start, e
         alpha_stride = alpha.stride(0) if alpha.numel() > 1 else 0
     if x.rows == 0 or w.rows == 0:
         return
+    args = _lib.BLOCK_SCALED_GEMM_ARGS.pack(
+        x.data.data_ptr(), x.row_stride, x.sf.data_ptr(), x.sf_strides[1], x.sf_strides[2], x.block_m, x.block_k, w.data.data_ptr(), w.group_stride,
+        w.row_stride, w.sf.data_ptr(), *w.sf_strides, w.block_m, w.block_k, x.fmt, x.sf_fmt, 0 if expert_start is None else expert_start.data_ptr(),
+        0 if expert_end is None else expert_end.data_ptr(), num_experts, x.rows, w.rows, x.k, alpha_ptr, alpha_stride, out.data_ptr(),
+        out.stride(0), flags)
     device = out.device
     with device_guard(device):
-        rc = _lib.lib().tkq_block_scaled_gemm(
-            x.data.data_ptr(), x.row_stride, x.sf.data_ptr(), x.sf_strides[1], x.sf_strides[2], x.block_m, x.block_k, w.data.data_ptr(),
-            w.group_stride, w.row_stride, w.sf.data_ptr(), *w.sf_strides, w.block_m, w.block_k, x.fmt, x.sf_fmt,
-            None if expert_start is None else expert_start.data_ptr(), None if expert_end is None else expert_end.data_ptr(),
-            num_experts, x.rows, w.rows, x.k, alpha_ptr, alpha_stride, out.data_ptr(), out.stride(0), flags, current_stream_ptr(device))
+        rc = _lib.lib().tkq_block_scaled_gemm(args, current_stream_ptr(device))
     if rc:
         _lib.check(rc, 'tkq_block_scaled_gemm')
 
@@ -115,7 +116,7 @@ def block_scaled_gemm(
     x, w = ScaledOperand(a, a_block_size, None), ScaledOperand(b, b_block_size, None)
     shape = (x.rows, w.rows)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=x.data.device)
+        out = empty_matrix(x.rows, w.rows, torch.bfloat16, x.data.device)
     else:
         check_out(out, shape, x.data)
     launch_block_scaled_gemm(x, w, None, None, 1, alpha, out, 0)

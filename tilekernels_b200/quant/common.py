@@ -181,6 +181,11 @@ def current_stream_ptr(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def empty_matrix(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """torch.empty((rows, cols)) by the call that takes two thirds of its host time (1.5 us)."""
+    return torch.empty_strided((rows, cols), (max(cols, 1), 1), dtype=dtype, device=device)
+
+
 _NO_GUARD = contextlib.nullcontext()
 
 
@@ -188,7 +193,7 @@ def device_guard(device: torch.device):
     """Context that makes `device` current for the C call.  Switching and restoring the device costs several
     microseconds per call, more than a third of a small cast's wrapper time: nothing is switched when `device` is
     current already, which is the usual case."""
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _NO_GUARD if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 _E2M1_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)

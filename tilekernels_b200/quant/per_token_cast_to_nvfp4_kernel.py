@@ -3,7 +3,7 @@ cast_back calls.  The reference's FP4 cast has power-of-two scales only (tile_ke
 import torch
 
 from .. import _lib
-from .common import DTYPE_TO_ENUM, current_stream_ptr, device_guard
+from .common import DTYPE_TO_ENUM, current_stream_ptr, device_guard, empty_matrix
 from .types import QuantTensor
 
 
@@ -33,8 +33,9 @@ def per_token_cast_to_nvfp4(x: torch.Tensor, tensor_scale: torch.Tensor) -> Quan
     num_tokens, hidden = x.shape
     assert hidden > 0 and hidden % 16 == 0 and x.stride(1) == 1
     _check_tensor_scale(tensor_scale, x.device)
-    out = torch.empty((num_tokens, hidden // 2), dtype=torch.int8, device=x.device)
-    out_sf = torch.empty((num_tokens, hidden // 16), dtype=torch.float8_e4m3fn, device=x.device)
+    device = x.device
+    out = empty_matrix(num_tokens, hidden // 2, torch.int8, device)
+    out_sf = empty_matrix(num_tokens, hidden // 16, torch.float8_e4m3fn, device)
     if num_tokens > 0:
         with device_guard(x.device):
             rc = _lib.lib().tkq_per_token_cast_nvfp4(x.data_ptr(), DTYPE_TO_ENUM[x.dtype], num_tokens, hidden, x.stride(0),
@@ -52,7 +53,7 @@ def cast_back_nvfp4(x: QuantTensor, fmt: str, tensor_scale: torch.Tensor) -> tor
     assert hidden > 0 and hidden % 16 == 0
     assert sf.dtype == torch.float8_e4m3fn and sf.shape == (num_tokens, hidden // 16) and sf.is_contiguous() and sf.get_device() == data.get_device()
     _check_tensor_scale(tensor_scale, data.device)
-    out = torch.empty((num_tokens, hidden), dtype=torch.bfloat16 if fmt == 'bf16' else torch.float32, device=data.device)
+    out = empty_matrix(num_tokens, hidden, torch.bfloat16 if fmt == 'bf16' else torch.float32, data.device)
     if num_tokens > 0:
         with device_guard(data.device):
             rc = _lib.lib().tkq_cast_back_nvfp4(data.data_ptr(), sf.data_ptr(), tensor_scale.data_ptr(), num_tokens, hidden,
