@@ -114,6 +114,17 @@ def test_alpha_out_and_strides(cuda_device, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('fmt,block', (('e4m3', (128, 128)), ('e4m3', (32, 32)), ('e4m3', (32, 128)), ('e2m1', (32, 32)), ('e2m1', (128, 32))))
+@pytest.mark.parametrize('m', (7, 130, 400))
+def test_scales_of_row_blocks_in_the_left_operand(cuda_device, fmt, block, m):
+    from tilekernels_b200 import quant
+    a, b = _matrices(m, 200, 576, cuda_device)
+    other = (1, 128) if fmt == 'e4m3' else (1, 32)
+    (qa, va, _), (qb, vb, _) = quantize(a, fmt, block), quantize(b, fmt, other)
+    assert_product(quant.block_scaled_gemm(qa, qb, block, other), va, vb)
+
+
+@pytest.mark.gpu
 def test_extreme_scales_and_special_codes(cuda_device):
     """Scales of 2^-60 .. 2^60 in either operand, and rows whose NaN reaches their own results only."""
     from tilekernels_b200 import quant
