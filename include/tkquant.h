@@ -2,7 +2,7 @@
  * tkquant.h -- C ABI of libtkquant.so: B200 (sm_100a) quantization casts.
  *
  * Every entry point takes plain device pointers and sizes, enqueues exactly one
- * kernel on `stream` (a cudaStream_t passed as void*; NULL = the legacy default
+ * kernel (or, for a weight gradient without rows, one memset) on `stream` (a cudaStream_t passed as void*; NULL = the legacy default
  * stream) and returns without synchronising.  Nothing here allocates, frees or
  * keeps a pointer after the launch.
  *
@@ -73,7 +73,8 @@ const char* tkq_last_error_string(void);
  * flags could not be read.  No counterpart in the reference.
  *
  *   TKQ_DEVICE_WAIT_TIMEOUT   a kernel that waits for asynchronous copies into shared memory (the per-block and
- *                             per-channel tile kernels, the E5M6 row pipeline, the staged SwiGLU cast) ran out of
+ *                             per-channel tile kernels, the E5M6 row pipeline, the staged SwiGLU cast), or a matrix
+ *                             product whose warps wait for one another, ran out of
  *                             polls (a limit that is seconds long), and returned early.  Outputs of that launch
  *                             are undefined: rows or tiles may be missing or partly written.
  *   TKQ_DEVICE_LOSSLESS_RANGE tkq_per_block_cast_lossless met an input scale more than 2^5 below its output

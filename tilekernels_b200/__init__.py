@@ -1,7 +1,8 @@
 """tilekernels_b200 -- B200 (sm_100a) implementation of the TileKernels quantization casts.
 
 `tilekernels_b200.quant` exposes the entry points of the reference's `tile_kernels.quant`
-hot path under the same names, argument lists and return conventions.  Every call
+hot path under the same names, argument lists and return conventions, and beside them the matrix
+products that read quantized tensors (`quant.block_scaled_gemm`, `moe.grouped_gemm`).  Every call
 ends in one hand-written CUDA kernel of libtkquant.so (C ABI, see include/tkquant.h);
 there is no other backend and no CPU path: importing `quant` without the built
 library raises.

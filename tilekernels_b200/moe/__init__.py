@@ -1,6 +1,6 @@
-"""The one MoE entry point next to the quantization path: row expansion with scale factors
-(reference: tile_kernels/moe/__init__.py, expand_to_fused_kernel.py).  The rest of the reference's moe package
-(gating, mapping, reduction) is outside this library."""
+"""MoE entry points next to the quantization path: row expansion with scale factors (reference: tile_kernels/moe/__init__.py,
+expand_to_fused_kernel.py) and the products grouped by expert that its rows are laid out for.  The rest of the reference's
+moe package (gating, mapping, reduction) is outside this library."""
 from .. import _lib as _lib_module
 
 _lib_module.lib()  # fail at import when the CUDA library is missing
