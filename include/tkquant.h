@@ -394,9 +394,19 @@ int tkq_block_scaled_gemm(const tkq_block_scaled_gemm_args* args, void* stream);
  *
  *   x    [num_rows, k] bf16;  w  [num_experts, n, k], with transpose_w [num_experts, k, n]; rows on 16-byte boundaries
  */
-int tkq_grouped_gemm(const void* x, int64_t x_row_stride, const void* w, int64_t w_expert_stride, int64_t w_row_stride,
-                     int transpose_w, const int32_t* expert_start, const int32_t* expert_end, int64_t num_experts,
-                     int64_t num_rows, int64_t n, int64_t k, void* out, int64_t out_row_stride, unsigned flags, void* stream);
+typedef struct tkq_grouped_gemm_args { /* 8-byte fields only */
+    const void* x;
+    int64_t x_row_stride;
+    const void* w;
+    int64_t w_expert_stride, w_row_stride, transpose_w;
+    const int32_t* expert_start;
+    const int32_t* expert_end;
+    int64_t num_experts, num_rows, n, k;
+    void* out;
+    int64_t out_row_stride, flags;
+} tkq_grouped_gemm_args;
+
+int tkq_grouped_gemm(const tkq_grouped_gemm_args* args, void* stream);
 
 /*
  * Gradient of each expert's weight: out[e, j, i] (+)= sum over the rows r of group e of grad[r, j] * x[r, i], fp32 sums.
@@ -406,9 +416,19 @@ int tkq_grouped_gemm(const void* x, int64_t x_row_stride, const void* w, int64_t
  *   grad  [num_rows, n] bf16;  x  [num_rows, k] bf16; rows on 16-byte boundaries
  *   out   [num_experts, n, k] contiguous, bf16 or fp32 (out_dtype); TKQ_ACCUMULATE needs fp32
  */
-int tkq_grouped_gemm_wgrad(const void* grad, int64_t grad_row_stride, const void* x, int64_t x_row_stride,
-                           const int32_t* expert_start, const int32_t* expert_end, int64_t num_experts, int64_t num_rows,
-                           int64_t n, int64_t k, int out_dtype, void* out, unsigned flags, void* stream);
+typedef struct tkq_grouped_gemm_wgrad_args { /* 8-byte fields only */
+    const void* grad;
+    int64_t grad_row_stride;
+    const void* x;
+    int64_t x_row_stride;
+    const int32_t* expert_start;
+    const int32_t* expert_end;
+    int64_t num_experts, num_rows, n, k, out_dtype;
+    void* out;
+    int64_t flags;
+} tkq_grouped_gemm_wgrad_args;
+
+int tkq_grouped_gemm_wgrad(const tkq_grouped_gemm_wgrad_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -36,19 +36,26 @@ def test_argument_checks_of_the_products(lib):
     assert call(flags=1) == -2
     assert call(x=p16 + 8) == -3 and call(xs=136) == -3 and call(x_sf=p16 + 2) == -3 and call(out=p16 + 1) == -3
     assert b'block_scaled_gemm' in lib.tkq_last_error_string()
-    grouped = lib.tkq_grouped_gemm
-    # (x, row stride, w, expert stride, row stride, transpose, start, end, experts, rows, n, k, out, out stride, flags, stream)
-    assert grouped(p16, 64, p16, 4096, 64, 0, p16, p16, 2, 0, 64, 64, p16, 64, 0, None) == 0
-    assert grouped(p16, 64, p16, 4096, 64, 0, None, None, 1, 4, 64, 64, p16, 64, 0, None) == -1
-    assert grouped(p16, 60, p16, 4096, 64, 0, p16, p16, 2, 4, 64, 64, p16, 64, 0, None) == -3
-    assert grouped(p16, 64, p16, 4096, 64, 0, p16, p16, 2, 4, 64, 64, p16, 64, 128, None) == -2
-    wgrad = lib.tkq_grouped_gemm_wgrad
-    # (grad, row stride, x, row stride, start, end, experts, rows, n, k, dtype, out, flags, stream)
-    assert wgrad(p16, 64, p16, 64, p16, p16, 2, 0, 64, 64, 1, p16, 128, None) == 0   # accumulate nothing
-    assert wgrad(p16, 64, p16, 64, p16, p16, 2, 4, 64, 64, 2, p16, 0, None) == -1    # output type
-    assert wgrad(p16, 64, p16, 64, p16, p16, 2, 4, 64, 64, 0, p16, 128, None) == -2  # accumulation in bf16
-    assert wgrad(p16, 64, p16, 64, None, p16, 2, 4, 64, 64, 1, p16, 0, None) == -1
-    assert wgrad(p16 + 2, 64, p16, 64, p16, p16, 2, 4, 64, 64, 1, p16, 0, None) == -3
+    # (x, row stride, w, expert stride, row stride, transpose, start, end, experts, rows, n, k, out, out stride, flags)
+    def grouped(*args):
+        return lib.tkq_grouped_gemm(_lib.GROUPED_GEMM_ARGS.pack(*args), None)
+
+    assert lib.tkq_grouped_gemm(None, None) == -1
+    assert grouped(p16, 64, p16, 4096, 64, 0, p16, p16, 2, 0, 64, 64, p16, 64, 0) == 0
+    assert grouped(p16, 64, p16, 4096, 64, 0, 0, 0, 1, 4, 64, 64, p16, 64, 0) == -1
+    assert grouped(p16, 60, p16, 4096, 64, 0, p16, p16, 2, 4, 64, 64, p16, 64, 0) == -3
+    assert grouped(p16, 64, p16, 4096, 64, 0, p16, p16, 2, 4, 64, 64, p16, 64, 128) == -2
+
+    # (grad, row stride, x, row stride, start, end, experts, rows, n, k, dtype, out, flags)
+    def wgrad(*args):
+        return lib.tkq_grouped_gemm_wgrad(_lib.GROUPED_GEMM_WGRAD_ARGS.pack(*args), None)
+
+    assert lib.tkq_grouped_gemm_wgrad(None, None) == -1
+    assert wgrad(p16, 64, p16, 64, p16, p16, 2, 0, 64, 64, 1, p16, 128) == 0   # accumulate nothing
+    assert wgrad(p16, 64, p16, 64, p16, p16, 2, 4, 64, 64, 2, p16, 0) == -1    # output type
+    assert wgrad(p16, 64, p16, 64, p16, p16, 2, 4, 64, 64, 0, p16, 128) == -2  # accumulation in bf16
+    assert wgrad(p16, 64, p16, 64, 0, p16, 2, 4, 64, 64, 1, p16, 0) == -1
+    assert wgrad(p16 + 2, 64, p16, 64, p16, p16, 2, 4, 64, 64, 1, p16, 0) == -3
     assert b'grouped_gemm_wgrad' in lib.tkq_last_error_string()
 
 

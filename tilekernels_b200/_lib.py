@@ -39,13 +39,15 @@ SIGNATURES = {
     'tkq_expand_to_fused': [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _uint, _vp, _vp, _i64, _vp],
     'tkq_per_token_cast_nvfp4': [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp],
     'tkq_cast_back_nvfp4': [_vp, _vp, _vp, _i64, _i64, _int, _vp, _vp],
-    'tkq_block_scaled_gemm': [ctypes.c_char_p, _vp],  # BLOCK_SCALED_GEMM_ARGS.pack(...), stream
-    'tkq_grouped_gemm': [_vp, _i64, _vp, _i64, _i64, _int, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _uint, _vp],
-    'tkq_grouped_gemm_wgrad': [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp, _uint, _vp],
+    'tkq_block_scaled_gemm': [ctypes.c_char_p, _vp],  # the packed arguments below, stream
+    'tkq_grouped_gemm': [ctypes.c_char_p, _vp],
+    'tkq_grouped_gemm_wgrad': [ctypes.c_char_p, _vp],
 }
 
-# tkq_block_scaled_gemm_args: converting as many arguments one by one takes ctypes 3 us, packing them 0.3 us
+# The argument structs of the products.  Converting 29 arguments one by one takes ctypes 3 us, packing them 0.3 us.
 BLOCK_SCALED_GEMM_ARGS = struct.Struct('@29q')
+GROUPED_GEMM_ARGS = struct.Struct('@15q')
+GROUPED_GEMM_WGRAD_ARGS = struct.Struct('@13q')
 
 _lib = None
 

@@ -203,11 +203,13 @@ extern "C" int tkq_block_scaled_gemm(const tkq_block_scaled_gemm_args* args, voi
     return launch_rows<kKindNvf4, 96, 224, false>(a, b, p, "block_scaled_gemm", s);
 }
 
-extern "C" int tkq_grouped_gemm(const void* x, int64_t x_row_stride, const void* w, int64_t w_expert_stride, int64_t w_row_stride, int transpose_w,
-                                const int32_t* expert_start, const int32_t* expert_end, int64_t num_experts, int64_t num_rows, int64_t n,
-                                int64_t k, void* out, int64_t out_row_stride, unsigned flags, void* stream) {
+extern "C" int tkq_grouped_gemm(const tkq_grouped_gemm_args* args, void* stream) {
+    static_assert(sizeof(tkq_grouped_gemm_args) == 15 * 8, "8-byte fields only");
+    if (args == nullptr) return set_error(TKQ_E_BAD_ARG, "grouped_gemm: null pointer");
+    const auto [x, x_row_stride, w, w_expert_stride, w_row_stride, transpose_w, expert_start, expert_end, num_experts, num_rows, n, k, out,
+                out_row_stride, flags] = *args;
     if (int rc = check_sizes(num_experts, num_rows, n, k)) return rc;
-    if (flags & ~static_cast<unsigned>(TKQ_ZERO_GAPS)) return set_error(TKQ_E_UNSUPPORTED, "grouped_gemm: only TKQ_ZERO_GAPS applies");
+    if (flags & ~int64_t{TKQ_ZERO_GAPS}) return set_error(TKQ_E_UNSUPPORTED, "grouped_gemm: only TKQ_ZERO_GAPS applies");
     if (num_rows == 0) return 0;
     if (x == nullptr || w == nullptr || out == nullptr || expert_start == nullptr || expert_end == nullptr)
         return set_error(TKQ_E_BAD_ARG, "grouped_gemm: null pointer");
@@ -231,12 +233,13 @@ extern "C" int tkq_grouped_gemm(const void* x, int64_t x_row_stride, const void*
     return launch_rows<kKindBf16, 128, 256, false>(a, b, p, "grouped_gemm", s);
 }
 
-extern "C" int tkq_grouped_gemm_wgrad(const void* grad, int64_t grad_row_stride, const void* x, int64_t x_row_stride, const int32_t* expert_start,
-                                      const int32_t* expert_end, int64_t num_experts, int64_t num_rows, int64_t n, int64_t k, int out_dtype,
-                                      void* out, unsigned flags, void* stream) {
+extern "C" int tkq_grouped_gemm_wgrad(const tkq_grouped_gemm_wgrad_args* args, void* stream) {
+    static_assert(sizeof(tkq_grouped_gemm_wgrad_args) == 13 * 8, "8-byte fields only");
+    if (args == nullptr) return set_error(TKQ_E_BAD_ARG, "grouped_gemm_wgrad: null pointer");
+    const auto [grad, grad_row_stride, x, x_row_stride, expert_start, expert_end, num_experts, num_rows, n, k, out_dtype, out, flags] = *args;
     if (int rc = check_sizes(num_experts, num_rows, n, k)) return rc;
     if (out_dtype != TKQ_DT_BF16 && out_dtype != TKQ_DT_FP32) return set_error(TKQ_E_BAD_ARG, "grouped_gemm_wgrad: unknown output type");
-    if (flags & ~static_cast<unsigned>(TKQ_ACCUMULATE)) return set_error(TKQ_E_UNSUPPORTED, "grouped_gemm_wgrad: only TKQ_ACCUMULATE applies");
+    if (flags & ~int64_t{TKQ_ACCUMULATE}) return set_error(TKQ_E_UNSUPPORTED, "grouped_gemm_wgrad: only TKQ_ACCUMULATE applies");
     if ((flags & TKQ_ACCUMULATE) && out_dtype != TKQ_DT_FP32)
         return set_error(TKQ_E_UNSUPPORTED, "grouped_gemm_wgrad: accumulation needs a float32 output");
     if (out == nullptr || expert_start == nullptr || expert_end == nullptr || (num_rows > 0 && (grad == nullptr || x == nullptr)))

@@ -75,10 +75,10 @@ def grouped_gemm(
     if quantized:
         launch_block_scaled_gemm(xo, wo, expert_start, expert_end, num_experts, alpha, out, flags)
     elif num_rows > 0 and n > 0:
+        args = _lib.GROUPED_GEMM_ARGS.pack(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w.stride(1), int(transpose_w), expert_start.data_ptr(),
+                                           expert_end.data_ptr(), num_experts, num_rows, n, k, out.data_ptr(), out.stride(0), flags)
         with device_guard(device):
-            rc = _lib.lib().tkq_grouped_gemm(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w.stride(1), int(transpose_w),
-                                             expert_start.data_ptr(), expert_end.data_ptr(), num_experts, num_rows, n, k, out.data_ptr(),
-                                             out.stride(0), flags, current_stream_ptr(device))
+            rc = _lib.lib().tkq_grouped_gemm(args, current_stream_ptr(device))
         if rc:
             _lib.check(rc, 'tkq_grouped_gemm')
     return out
@@ -116,15 +116,16 @@ def grouped_gemm_wgrad(
     device = x.device
     if out is None:
         assert not accumulate, 'accumulate needs out'
-        out = torch.empty((num_experts, n, k), dtype=out_dtype, device=device)
+        out = torch.empty_strided((num_experts, n, k), (max(n * k, 1), max(k, 1), 1), dtype=out_dtype, device=device)
     else:
         assert out.shape == (num_experts, n, k) and out.dtype is out_dtype and out.get_device() == x.get_device() and out.is_contiguous()
         assert not accumulate or out_dtype is torch.float32, 'accumulate needs a float32 destination'
     if n > 0 and k > 0:
+        args = _lib.GROUPED_GEMM_WGRAD_ARGS.pack(grad.data_ptr(), grad.stride(0), x.data_ptr(), x.stride(0), expert_start.data_ptr(), expert_end.data_ptr(),
+                                                 num_experts, num_rows, n, k, DTYPE_TO_ENUM[out_dtype], out.data_ptr(),
+                                                 _lib.ACCUMULATE if accumulate else 0)
         with device_guard(device):
-            rc = _lib.lib().tkq_grouped_gemm_wgrad(grad.data_ptr(), grad.stride(0), x.data_ptr(), x.stride(0), expert_start.data_ptr(),
-                                                   expert_end.data_ptr(), num_experts, num_rows, n, k, DTYPE_TO_ENUM[out_dtype],
-                                                   out.data_ptr(), _lib.ACCUMULATE if accumulate else 0, current_stream_ptr(device))
+            rc = _lib.lib().tkq_grouped_gemm_wgrad(args, current_stream_ptr(device))
         if rc:
             _lib.check(rc, 'tkq_grouped_gemm_wgrad')
     return out
