@@ -360,8 +360,8 @@ int tkq_cast_back_nvfp4(const void* x, const void* sf, const float* tensor_scale
  *   *_block_m        rows per scale: 1, 32 or 128;  *_block_k values per scale: 32 or 128 (e4m3), 32 (e2m1, ue8m0),
  *                    16 (e2m1, e4m3 scales)
  *   fmt, sf_fmt      TKQ_FMT_E4M3 or TKQ_FMT_E2M1; TKQ_SFMT_UE8M0, or TKQ_SFMT_E4M3 with e2m1
- *   expert_start/end int32[num_experts], ascending and disjoint; values outside [0, num_rows] are clamped.  Both NULL with
- *                    num_experts = 1: one group of all rows
+ *   expert_start/end int32[num_experts], ascending and disjoint; values outside [0, num_rows] are clamped, and a group has
+ *                    no rows before the end of an earlier one.  Both NULL with num_experts = 1: one group of all rows
  *   k                multiple of 32 (e4m3) or 64 (e2m1); data rows start on 16-byte boundaries
  *   alpha            NULL or fp32, alpha[e * alpha_stride]
  *   out              bf16 [num_rows, out_row_stride]; rows of no group are left alone, or cleared with TKQ_ZERO_GAPS

@@ -196,6 +196,34 @@ def test_bounds_outside_the_rows_are_clamped(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('start,end,mine', (
+    ((0, 5, 5), (10, 20, 12), ((0, 10), (10, 20), (20, 20))),           # overlapping
+    ((12, 0, 14), (14, 8, 30), ((12, 14), (14, 14), (14, 30))),         # out of order
+    ((40, -7, 3), (50, -9, 2), ((30, 30), (30, 30), (30, 30))),         # outside, ends before starts
+    ((25, 0, 30, 10), (4, 10, 30, 20), ((0, 0), (0, 10), (10, 10), (10, 20))),  # experts without rows point elsewhere
+    ((0,) * 40, (30,) * 40, ((0, 30),) + ((30, 30),) * 39),             # all the same
+), ids=('overlapping', 'out of order', 'outside', 'empty', 'the same'))
+def test_segments_that_overlap_or_go_back(cuda_device, start, end, mine):
+    from tilekernels_b200 import moe
+    x, _, _, _ = _rows((30,), 64, cuda_device, spare=0)
+    w = torch.randn((len(start), 48, 64), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(cuda_device)
+    s, e = int32(start, cuda_device), int32(end, cuda_device)
+    first, last = zip(*mine)
+    got = moe.grouped_gemm(x, w, s, e)
+    _check_groups(got, x.cpu().double(), w.cpu().double(), first, last)
+    member = torch.zeros(30, dtype=torch.bool)
+    for a, b in mine:
+        member[a:b] = True
+    assert (got[~member.to(cuda_device)] == 0).all()
+    dw = moe.grouped_gemm_wgrad(x, x, s, e)
+    for i, (a, b) in enumerate(mine):
+        if a == b:
+            assert (dw[i] == 0).all()
+        else:
+            assert_product(dw[i], x[a:b].cpu().double().T, x[a:b].cpu().double().T)
+
+
+@pytest.mark.gpu
 def test_strided_operands(cuda_device):
     from tilekernels_b200 import moe
     sizes, n, k = (33, 0, 90), 136, 72

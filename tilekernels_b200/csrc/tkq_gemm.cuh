@@ -7,23 +7,20 @@
 //   weight grad i = input feature,  j = output feature, k = row            A = rows, B = their gradients
 //
 // The tensor core's M axis (128 lanes of tensor memory per CTA) carries i and its N axis carries j, whichever operand is
-// the weight.  Two things follow: a thread of the epilogue owns one i, so a warp's store of one row of the output is a
-// contiguous segment and needs no staging; and the ragged axis (rows of an expert) lies on N, whose extent an
-// instruction chooses in steps of 16, so that a group of a few rows costs no full tile.
+// the weight, so that the ragged axis (rows of an expert) lies on N, whose extent an instruction chooses in steps of 16: a
+// group of a few rows costs no full tile.  A warp of the epilogue has 32 neighbouring columns of the output in its lanes.
 //
 // A block: warp 0 loads operand tiles by TMA into a ring of stages, warp 1 issues the matrix instructions (accumulators in
-// tensor memory, two of them, so that one is drained while the other fills), warps 2 and 3 bring scale factors into the
-// layout the tensor core copies them from (or, for the weight gradient, clear the rows behind a group's end), warps 4 to
-// 7 store results.  Blocks are persistent and take tiles in turn.  With CG = 2 two CTAs on neighbouring SMs work on one
-// tile of 256 x N: each holds half of A's and half of B's rows, which halves the shared-memory fill per product.
+// tensor memory, two of them, so that one is drained while the other fills), the next warps bring scale factors into the
+// layout the tensor core copies them from (or, for the weight gradient, clear the rows behind a group's end), the last four
+// or eight store results.  Blocks are persistent and take tiles in turn.  With CG = 2 two CTAs on neighbouring SMs work on
+// one tile of 256 x N: each holds half of A's and half of B's rows, which halves the shared-memory fill per product.
 //
 // With few tiles (one token through one matrix) K is split over a cluster of CTAs: each multiplies its part of K, hands
 // its sums to the CTAs that own the columns, through their shared memory, and those add them in the order of the parts.
 #pragma once
 
 #include <cuda_bf16.h>
-
-#include <type_traits>
 
 #include "tkq_launch.cuh"
 #include "tkq_tcgen05.cuh"
@@ -40,7 +37,7 @@ struct ScaleView {
     int64_t group_stride, row_stride, k_stride;
     uint32_t row_shift;
     uint32_t words;      // words along K
-    uint32_t k_shift;    // 2: a byte covers 128 values (one word per four stages), 0: 32 or 16 values
+    uint32_t k_shift;    // 2: a byte covers 128 values (one word for two stages), 0: 32 or 16 values
     uint32_t vec;        // the words of a row lie together on 32-byte boundaries
 };
 
@@ -109,7 +106,7 @@ struct GemmConfig {
 
 // A tile's rows of B come in one box.  The last tile of a group often has few rows, and loads, which bound the products of
 // 256 x N tiles as much as the tensor core does, then take a box of a half or a quarter (16 experts of skewed sizes, bf16:
-// MEASURE).  Several small boxes instead of a large one are slower (312 -> 360 us on 8192 x 4096 x 7168).
+// 386 -> 383 us, NVFP4 55.8 -> 55.5).  Several small boxes instead of a large one are slower (312 -> 360 us on 8192 x 4096 x 7168).
 struct GemmMapsB {
     CUtensorMap box[3];
 };
@@ -369,19 +366,33 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             prefetch_tensor_map(&map_a);
             prefetch_tensor_map(&maps_b.box[0]);
         }
-        // group table: start and rows clamped to the tensor, tiles before each group
-        uint32_t before = 0;
+        // Group table: start and rows, clamped to the tensor and to what lies behind all earlier groups (so that every row is in one
+        // group at most, whatever the bounds say), and the tiles before each group.  A group without rows ends nothing.
+        uint32_t before = 0, taken = 0;
         for (uint32_t e0 = 0; e0 < p.groups; e0 += 32) {
             const uint32_t e = e0 + lane;
-            uint32_t tiles = 0;
+            uint32_t tiles = 0, first = 0, last = 0;
             if (e < p.groups) {
-                int64_t s = 0, t = p.rows;
+                last = p.rows;
                 if (p.start != nullptr) {
-                    s = min(max(static_cast<int64_t>(p.start[e]), int64_t{0}), static_cast<int64_t>(p.rows));
-                    t = min(max(static_cast<int64_t>(p.end[e]), s), static_cast<int64_t>(p.rows));
+                    first = static_cast<uint32_t>(min(max(static_cast<int64_t>(p.start[e]), int64_t{0}), static_cast<int64_t>(p.rows)));
+                    last = static_cast<uint32_t>(min(max(static_cast<int64_t>(p.end[e]), int64_t{0}), static_cast<int64_t>(p.rows)));
+                    if (last <= first) last = 0;
                 }
-                const uint32_t rows = static_cast<uint32_t>(t - s);
-                s_start[e] = static_cast<uint32_t>(s);
+            }
+            uint32_t end = max(last, taken);  // the largest end so far
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(kFullMask, end, o);
+                if (lane >= o) end = max(end, up);
+            }
+            uint32_t earlier = __shfl_up_sync(kFullMask, end, 1);
+            if (lane == 0) earlier = taken;
+            taken = __shfl_sync(kFullMask, end, 31);
+            if (e < p.groups) {
+                first = max(first, earlier);
+                const uint32_t rows = last > first ? last - first : 0;
+                s_start[e] = min(first, end);
                 s_rows[e] = rows;
                 tiles = (rows + C::NMAX - 1) / C::NMAX * p.i_tiles;
             }

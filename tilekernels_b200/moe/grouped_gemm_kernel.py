@@ -39,7 +39,8 @@ def grouped_gemm(
             gives the gradient of the input.  Or a quantized pair: data (num_experts, n, k), scales
             (num_experts, blocks of rows, words) or, for whole blocks, one matrix of all experts' rows.
         expert_start, expert_end: int32 (num_experts,), ascending; segments may be empty, of any length and alignment, and
-            need not touch.  At most 1024 experts.
+            need not touch.  Where they overlap or go back, an expert has no rows before the end of an earlier one.  At most
+            1024 experts.
         x_block_size, w_block_size: (rows, values) per scale of quantized operands, as in quant.block_scaled_gemm.
         alpha: optional fp32 tensor with one factor for all or one per expert (quantized operands).
         out: optional (num_rows, n) bfloat16 destination with unit column stride.  Rows of no expert are left as they
