@@ -140,6 +140,35 @@ def test_wgrad(cuda_device, name, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('sizes,n,k', (
+    ((4100,), 128, 128), ((4100,), 8, 264), ((20000,), 136, 8),
+    ((63, 2000, 0, 513, 1), 300, 136), ((0, 0, 9000, 0), 128, 256),   # parts without rows, experts without rows
+    ((0,), 128, 128), ((700, 1, 650) * 20, 128, 128), ((300,) * 37, 256, 256),
+    ((800, 500), 1024, 1024),
+), ids=str)
+def test_wgrad_of_small_weights(cuda_device, sizes, n, k):
+    """Few tiles: the rows of a group are split over a cluster of blocks, whose sums are added in the order of the parts."""
+    from tilekernels_b200 import moe
+    # (rows start on 16-byte boundaries)
+    x, start, end, _ = _rows(sizes, -(-k // 8) * 8, cuda_device, gap=3, first=1)
+    g, _, _, _ = _rows(sizes, -(-n // 8) * 8, cuda_device, gap=3, first=1, seed=1)
+    x, g = x[:, :k], g[:, :n]
+    s, e = int32(start, cuda_device), int32(end, cuda_device)
+    for dtype in (torch.float32, torch.bfloat16):
+        got = moe.grouped_gemm_wgrad(g, x, s, e, out_dtype=dtype)
+        for i, (a, b) in enumerate(zip(start, end)):
+            if a == b:
+                assert (got[i] == 0).all()
+            else:
+                assert_product(got[i], g[a:b].cpu().double().T, x[a:b].cpu().double().T)
+        assert torch.equal(moe.grouped_gemm_wgrad(g, x, s, e, out_dtype=dtype), got)
+    before = torch.randn(got.shape, generator=torch.Generator().manual_seed(2)).to(cuda_device)
+    out = before.clone()
+    moe.grouped_gemm_wgrad(g, x, s, e, out=out, accumulate=True)
+    assert torch.equal(out, before + moe.grouped_gemm_wgrad(g, x, s, e))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('rows', (250, 1025, 9000))
 def test_wgrad_of_long_groups_keeps_its_precision(cuda_device, rows):
     """The tensor core's sum goes on in registers every 256 rows.  A step of 16 rows cuts off at most one unit (2^-23 of the

@@ -89,14 +89,22 @@ static int64_t row_tiles(const GemmParams& p, int nmax) {
     return p.groups == 1 ? (int64_t{p.rows} + nmax - 1) / nmax : int64_t{p.rows} / nmax + p.groups;
 }
 
-// Tiles that leave most SMs idle are split along K, over as many CTAs as there are SMs for; a cluster takes one tile.  One
-// row of FP8 through 4096 x 7168: 14.9 us whole, 10.5 us split by 4; of NVFP4 through 7168 x 2048 (eight stages): 7.8 us
-// whole, 8.4 us split by 2, so a part has at least six stages.
+// CTAs that share a tile along K: as many as there are SMs for, with at least `part` stages each.  Clusters of eight take half
+// the SMs at most: they have to fit into groups of SMs, and of sixteen the last ones run after the others (one row of bf16 through
+// 2048 x 7168: 18.5 us with sixteen clusters of eight, 13.7 of four).
+static uint32_t split_of(int64_t tiles, int64_t stages, int64_t part) {
+    const int64_t sms = device_sm_count();
+    uint32_t split = 1;
+    while (split < 8 && tiles * split * 2 <= (split == 4 ? sms / 2 : sms) && stages >= 2 * part * split) split *= 2;
+    return split;
+}
+
+// Tiles that leave most SMs idle are split along K; a cluster takes one tile.  One row of FP8 through 4096 x 7168: 14.9 us whole,
+// 10.5 us split by 4; of NVFP4 through 7168 x 2048 (eight stages): 7.8 us whole, 8.4 us split by 2, so a part has at least six.
 template <int KIND, int NMAX, bool A_MN>
 static bool launch_split(const Operand& a, const Operand& b, GemmParams p, const char* what, cudaStream_t stream, int* rc) {
     const int64_t tiles = row_tiles(p, NMAX) * ((p.i_size + 127) / 128);
-    p.split = 1;
-    while (p.split < 8 && tiles * p.split * 2 <= device_sm_count() && p.k_stages >= 12 * p.split) p.split *= 2;
+    p.split = split_of(tiles, p.k_stages, 6);
     if (p.split == 1) return false;
     *rc = launch_gemm<GemmConfig<KIND, 1, NMAX, false, A_MN, true>>(a, b, p, what, stream);
     return true;
@@ -266,6 +274,14 @@ extern "C" int tkq_grouped_gemm_wgrad(const tkq_grouped_gemm_wgrad_args* args, v
     p.j_size = static_cast<uint32_t>(n);
     p.accumulate = (flags & TKQ_ACCUMULATE) ? 1 : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // Small results whose 128 x 128 tiles leave SMs idle: the rows of a group are split over a cluster.  Whole (pairs on 256 x
+    // 256) against split: 20000 rows, 128 x 128: 102, 22 us; 4096 rows, 512 x 512: 27.5, 14.5; 8 experts, 16000 rows, 256 x 512:
+    // 25.5, 21.6.  Parts of five or six stages gained nothing (700 rows, 512 x 512: 10.6, 10.9), so a part has at least eight.
+    p.split = split_of(num_experts * ((n + 127) / 128) * ((k + 127) / 128), num_rows / num_experts / 64, 8);
+    if (p.split > 1) {
+        p.out_bf16 = out_dtype == TKQ_DT_BF16;
+        return launch_gemm<GemmConfig<kKindBf16, 1, 128, true, true, true, true>>(a, b, p, "grouped_gemm_wgrad", s);
+    }
     if (out_dtype == TKQ_DT_FP32) return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true, false, true>>(a, b, p, "grouped_gemm_wgrad", s);
     return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true>>(a, b, p, "grouped_gemm_wgrad", s);
 }

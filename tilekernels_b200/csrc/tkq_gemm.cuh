@@ -16,7 +16,7 @@
 // or eight store results.  Blocks are persistent and take tiles in turn.  With CG = 2 two CTAs on neighbouring SMs work on
 // one tile of 256 x N: each holds half of A's and half of B's rows, which halves the shared-memory fill per product.
 //
-// With few tiles (one token through one matrix) K is split over a cluster of CTAs: each multiplies its part of K, hands
+// With few tiles (one token through one matrix, the gradient of a small weight) K is split over a cluster of CTAs: each multiplies its part of K, hands
 // its sums to the CTAs that own the columns, through their shared memory, and those add them in the order of the parts.
 #pragma once
 
@@ -56,6 +56,7 @@ struct GemmParams {
     uint32_t alpha_stride;
     uint32_t split;  // CTAs of a cluster that share a tile along K
     uint32_t accumulate, zero_gaps;
+    uint32_t out_bf16;  // weight gradient split along K: bf16 results
     uint32_t wide_out;  // rows of out on 16-byte boundaries and i_size a multiple of 8
 };
 
@@ -80,7 +81,8 @@ struct GemmConfig {
     static constexpr uint32_t kFirstResultWarp = 2 + kLoaders, kResultWarps = F32 ? 8 : 4;
     static constexpr uint32_t kThreads = 32 * (kFirstResultWarp + kResultWarps);
     static constexpr uint32_t kStagingPerWarp = F32 ? 0 : SCALED ? 2048 : 4096, kStagingBytes = kStagingPerWarp * kResultWarps;
-    static constexpr uint32_t kPartialBytes = SPLIT ? NMAX * 128 * 4 : 0;
+    // split products: the parts' sums as [part][own column][row], columns padded so that 16-byte accesses meet no bank twice
+    static constexpr uint32_t kPartialPitch = NMAX + 4, kPartialBytes = SPLIT ? 128 * kPartialPitch * 4 : 0;
     // (NVFP4 with 224 rows: the scales leave room for three stages and a table of fewer groups)
     static constexpr uint32_t kGroups = KIND == kKindNvf4 && NMAX > 192 ? 96 : kMaxGroups;
     static constexpr uint32_t kFits = (kGemmSmemBudget - kStagingBytes - kPartialBytes - 12 * (kGroups + 1)) / kStageBytes;
@@ -96,7 +98,7 @@ struct GemmConfig {
     static constexpr uint32_t kNStep = CG == 2 ? 32 : 16;
     static_assert(kColsNeeded <= 512, "tensor memory");
     static_assert(kFirstResultWarp % 4 == 0, "a warp reads the quarter of tensor memory of its number modulo four");
-    static_assert(!SPLIT || (CG == 1 && !WGRAD), "the cluster of a split product is one along K");
+    static_assert(!SPLIT || (CG == 1 && (!WGRAD || F32)), "the cluster of a split product is one along K");
     static_assert(!WGRAD || (A_MN && kBRows % 64 == 0 && kSub == 1), "weight gradient reads both operands along their rows");
     static_assert(kBBytes % 1024 == 0, "stage layout");
     // A scale loader goes from stage `it` to `it` + kScaleSets.  It waits by parity, so the slot it comes to has to be at most one
@@ -296,6 +298,9 @@ __device__ __forceinline__ void store_bf16(const GemmParams& p, const GemmTile& 
     }
 }
 
+__device__ __forceinline__ uint32_t as_bits(uint32_t x) { return x; }
+__device__ __forceinline__ uint32_t as_bits(float x) { return __float_as_uint(x); }
+
 // fp32 results of the weight gradient.  The tensor core cuts off what an addition to its accumulator shifts out instead of
 // rounding, so a long sum drifts towards zero by about 2.3e-8 of itself per step of 16 rows (groups of some 900 rows: 1.3e-6
 // off).  Every 16 steps its sum is therefore added to one in registers, with rounding: eight warps hold 128 columns of the
@@ -336,6 +341,19 @@ __device__ __forceinline__ void store_f32(const GemmParams& p, const float (&sum
     }
 }
 
+// N rows from row j on of a lane's column i of the tile go to the CTA of the cluster that owns the column.  (Rows behind the
+// tile's last are never read.)
+template <class C, uint32_t N, class T>
+__device__ __forceinline__ void hand_over(const T (&v)[N], uint32_t j, uint32_t i, uint32_t split, uint32_t part, uint32_t partial) {
+    const uint32_t own = 128 / split;
+    const uint32_t to = map_to_rank(partial + ((part * own + i % own) * C::kPartialPitch + j) * 4, i / own);
+#pragma unroll
+    for (uint32_t q = 0; q < N; q += 4)
+        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + q * 4), "r"(as_bits(v[q])), "r"(as_bits(v[q + 1])),
+                     "r"(as_bits(v[q + 2])), "r"(as_bits(v[q + 3]))
+                     : "memory");
+}
+
 template <class C>
 __global__ void __launch_bounds__(C::kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ GemmMapsB maps_b, const GemmParams p) {
@@ -349,8 +367,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     const uint32_t unit = blockIdx.x / (C::SPLIT ? p.split : C::CG), units = gridDim.x / (C::SPLIT ? p.split : C::CG);
     // this CTA's part of K
     const uint32_t part = C::SPLIT ? cluster_rank() : 0;
-    const uint32_t k_first = C::SPLIT ? part * p.k_stages / p.split : 0;
+    const uint32_t k_first = C::SPLIT && !C::WGRAD ? part * p.k_stages / p.split : 0;
     const uint32_t k_end = C::SPLIT ? (part + 1) * p.k_stages / p.split : p.k_stages;
+
+    auto k_begin = [&](const GemmTile& tile) { return C::WGRAD && C::SPLIT ? part * tile.k_stages / p.split : k_first; };
+    auto k_stop = [&](const GemmTile& tile) { return !C::WGRAD ? k_end : C::SPLIT ? (part + 1) * tile.k_stages / p.split : tile.k_stages; };
 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t a_base = base, b_base = a_base + C::kStages * C::kSub * C::kABytes, staging = b_base + C::kStages * C::kSub * C::kBBytes;
@@ -449,10 +470,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             const GemmTile tile = sched.tile(p, t);
             const int32_t i0 = static_cast<int32_t>(tile.i0 + rank * 128u);
             const int32_t j0 = static_cast<int32_t>(tile.j0 + (C::CG == 2 ? rank * (tile.n_mma / 2) : 0));
-            const uint32_t k_last = C::WGRAD ? tile.k_stages : k_end;
+            const uint32_t k_from = k_begin(tile), k_last = k_stop(tile);
             const uint32_t small = C::kBoxes == 1 ? 0 : 4 * tile.n_mma <= C::NMAX ? 2 : 2 * tile.n_mma <= C::NMAX ? 1 : 0;
             const CUtensorMap* map_b = &maps_b.box[small];
-            for (uint32_t kb = k_first; kb < k_last; ++kb) {
+            for (uint32_t kb = k_from; kb < k_last; ++kb) {
                 ok = __any_sync(kFullMask, one && wait(bar(&empty_bar[s]), phase));
                 if (!ok) break;
                 const uint32_t a = a_base + s * (C::kSub * C::kABytes), b = b_base + s * (C::kSub * C::kBBytes);
@@ -510,15 +531,15 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             bool ok = true, ready = false;  // ready: the next stage's operands have been seen to be there
             for (uint32_t t = unit; ok && t < sched.total; t += units) {
                 const GemmTile tile = sched.tile(p, t);
-                const uint32_t k_last = C::WGRAD ? tile.k_stages : k_end;
-                if (k_last == 0) continue;
+                const uint32_t k_from = k_begin(tile), k_last = k_stop(tile);
+                if (k_last <= k_from) continue;
                 uint32_t a = 0, d = 0;
                 uint32_t idesc;
                 if constexpr (C::SCALED) idesc = idesc_scaled(kM, tile.n_mma, C::KIND == kKindMxf8 ? 0 : 1, C::KIND != kKindNvf4);
                 else idesc = idesc_bf16(kM, tile.n_mma, C::A_MN, C::WGRAD);
-                for (uint32_t kb = k_first; kb < k_last; ++kb) {
-                    const bool opens = kb == k_first || (C::F32 && kb % C::kChunk == 0);
-                    const bool closes = kb + 1 == k_last || (C::F32 && (kb + 1) % C::kChunk == 0);
+                for (uint32_t kb = k_from; kb < k_last; ++kb) {
+                    const bool opens = kb == k_from || (C::F32 && (kb - k_from) % C::kChunk == 0);
+                    const bool closes = kb + 1 == k_last || (C::F32 && (kb + 1 - k_from) % C::kChunk == 0);
                     if (opens) {
                         a = acc_it & 1u;
                         ok = __any_sync(kFullMask, one && wait(bar(&acc_empty[a]), ((acc_it >> 1) & 1u) ^ 1u));
@@ -535,7 +556,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                     bool seen = false;
                     if (one) seen = mbar_try_wait_cluster(bar(C::WGRAD ? &ready_bar[s] : &full_bar[s]), phase);
                     uint32_t n_units = 4 * C::kSub;
-                    if (kb + 1 == (C::WGRAD ? k_last : p.k_stages)) n_units = C::WGRAD ? (tile.k_rows - kb * 64 + 15) / 16 : p.last_units;
+                    if (kb + 1 == (C::WGRAD ? tile.k_stages : p.k_stages)) n_units = C::WGRAD ? (tile.k_rows - kb * 64 + 15) / 16 : p.last_units;
 #pragma unroll
                     for (uint32_t h = 0; h < C::kSub; ++h) {
                         if (h > 0 && 4 * h >= n_units) break;
@@ -631,7 +652,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 bool ok = true;
                 for (uint32_t t = unit; ok && t < sched.total; t += units) {
                     const GemmTile tile = sched.tile(p, t);
-                    for (uint32_t kb = 0; kb < tile.k_stages; ++kb) {
+                    for (uint32_t kb = k_begin(tile); kb < k_stop(tile); ++kb) {
                         ok = __any_sync(kFullMask, lane == 0 && wait(bar(&full_bar[s]), phase));
                         if (!ok) break;
                         const uint32_t valid = min(64u, tile.k_rows - kb * 64), padded = (valid + 15) / 16 * 16;
@@ -665,7 +686,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 float sum[128];
 #pragma unroll
                 for (uint32_t q = 0; q < 128; ++q) sum[q] = 0.0f;
-                for (uint32_t kb = 0; kb < tile.k_stages; kb += C::kChunk) {
+                for (uint32_t kb = k_begin(tile); kb < k_stop(tile); kb += C::kChunk) {
                     const uint32_t a = acc_it & 1u;
                     ok = __all_sync(kFullMask, wait(bar(&acc_full[a]), (acc_it >> 1) & 1u));
                     if (!ok) break;
@@ -677,7 +698,9 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                     if (lane == 0) mbar_arrive_cluster(leader_bar(&acc_empty[a]));
                 }
                 const uint32_t i = tile.i0 + rank * 128u + quarter * 32u + lane;
-                if (ok && i < p.i_size)
+                if constexpr (C::SPLIT) {
+                    if (ok && c < C::NMAX) hand_over<C>(sum, 0, quarter * 32 + lane, p.split, part, partial);
+                } else if (ok && i < p.i_size)
                     store_f32(p, sum, static_cast<float*>(p.out) + static_cast<int64_t>(tile.e) * p.out_group_stride +
                                           static_cast<int64_t>(tile.j0 + c) * p.out_stride + i, columns);
             }
@@ -702,12 +725,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 if constexpr (C::SPLIT) {
                     tmem_load32(taddr + c, v);
                     tmem_load_wait();
-                    // the owner of a column i keeps sums as [part][row j][its columns]
-                    const uint32_t own = 128 / p.split, i = quarter * 32 + lane;
-                    const uint32_t to = map_to_rank(partial + ((part * C::NMAX + c) * own + i % own) * 4, i / own);
-#pragma unroll
-                    for (uint32_t q = 0; q < 32; ++q)
-                        if (q < n) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + q * own * 4), "r"(v[q]) : "memory");
+                    hand_over<C>(v, c, quarter * 32 + lane, p.split, part, partial);
                 } else {
                     store_bf16<C>(p, tile, v, have, taddr + c, iw, c, n, alpha, stage_mem + (turn & 1u) * 2048u, lane);
                     if (C::kStagingPerWarp > 2048) ++turn;
@@ -747,18 +765,35 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     if constexpr (C::SPLIT) {
         if (unit < sched.total) {
             const GemmTile tile = sched.tile(p, unit);
+            if (C::WGRAD && tile.k_stages == 0 && p.accumulate) return;
             const float alpha = p.alpha == nullptr ? 1.0f : __ldg(p.alpha + static_cast<int64_t>(tile.e) * p.alpha_stride);
-            const uint32_t own = 128 / p.split;
-            for (uint32_t q = threadIdx.x; q < tile.jn * own; q += C::kThreads) {
-                const uint32_t j = q / own, i = tile.i0 + part * own + q % own;
-                float sum = 0.0f;
-                for (uint32_t from = 0; from < p.split; ++from) {
-                    float x;
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(partial + ((from * C::NMAX + j) * own + q % own) * 4));
-                    sum = __fadd_rn(sum, x);
+            const uint32_t own = 128 / p.split, log_own = 31 - __clz(own);
+            for (uint32_t q = threadIdx.x; q < (tile.jn + 3) / 4 << log_own; q += C::kThreads) {
+                const uint32_t col = q & (own - 1), j = (q >> log_own) * 4, i = tile.i0 + part * own + col;
+                if (i >= p.i_size) continue;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (uint32_t from = 0; from < 8; ++from) {
+                    if (from >= p.split) break;
+                    float x[4];
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+                                 : "r"(partial + ((from * own + col) * C::kPartialPitch + j) * 4));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sum[r] = __fadd_rn(sum[r], x[r]);
                 }
-                if (i < p.i_size)
-                    static_cast<__nv_bfloat16*>(p.out)[static_cast<int64_t>(tile.j0 + j) * p.out_stride + i] = __float2bfloat16_rn(__fmul_rn(sum, alpha));
+                int64_t at = (C::WGRAD ? static_cast<int64_t>(tile.e) * p.out_group_stride : 0) + static_cast<int64_t>(tile.j0 + j) * p.out_stride + i;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (j + r >= tile.jn) break;
+                    if (C::WGRAD && !p.out_bf16) {
+                        float* o = static_cast<float*>(p.out) + at;
+                        *o = p.accumulate ? __fadd_rn(*o, sum[r]) : sum[r];
+                    } else {
+                        static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(__fmul_rn(sum[r], alpha));
+                    }
+                    at += p.out_stride;
+                }
             }
         }
     }
