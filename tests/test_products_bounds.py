@@ -52,6 +52,47 @@ def test_products_write_their_output_only(cuda_device, rows, n):
             assert_product(out[1], g[rows // 2:].cpu().double().T, x[rows // 2:].cpu().double().T)
 
 
+@pytest.mark.parametrize('n,k', ((8, 8), (129, 131), (1, 300), (257, 5)))
+@pytest.mark.parametrize('dtype', (torch.float32, torch.bfloat16), ids=('fp32', 'bf16'))
+def test_split_weight_gradients_write_their_output_only(cuda_device, n, k, dtype):
+    """Long groups of a small weight, whose rows a cluster shares: eager, on two streams at once, and replayed with other bounds."""
+    from tilekernels_b200 import moe
+    gen = torch.Generator().manual_seed(n * k)
+    rows = 5000
+    g = torch.randn((rows, -(-n // 8) * 8), generator=gen).to(torch.bfloat16).to(cuda_device)[:, :n]
+    x = torch.randn((rows, -(-k // 8) * 8), generator=gen).to(torch.bfloat16).to(cuda_device)[:, :k]
+    s, e = int32([3, 1500], cuda_device), int32([1500, 4999], cuda_device)
+
+    def check_values(out, bounds):
+        for i, (a, b) in enumerate(bounds):
+            assert_product(out[i], g[a:b].cpu().double().T, x[a:b].cpu().double().T)
+
+    out, check = _guarded((2, n, k), dtype, cuda_device)
+    moe.grouped_gemm_wgrad(g, x, s, e, out_dtype=dtype, out=out)
+    check()
+    check_values(out, ((3, 1500), (1500, 4999)))
+    want = out.clone()
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(2)]
+    outs = [_guarded((2, n, k), dtype, cuda_device) for _ in streams]
+    torch.cuda.synchronize(cuda_device)
+    for _ in range(5):
+        for stream, (o, _) in zip(streams, outs):
+            with torch.cuda.stream(stream):
+                moe.grouped_gemm_wgrad(g, x, s, e, out_dtype=dtype, out=o)
+    torch.cuda.synchronize(cuda_device)
+    for o, c in outs:
+        c()
+        assert torch.equal(o, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        moe.grouped_gemm_wgrad(g, x, s, e, out_dtype=dtype, out=out)
+    s.copy_(int32([0, 4000], cuda_device))
+    e.copy_(int32([17, 5000], cuda_device))
+    graph.replay()
+    check()
+    check_values(out, ((0, 17), (4000, 5000)))
+
+
 @pytest.mark.parametrize('rows,hidden', ((1, 16), (3, 528), (129, 1040)))
 @pytest.mark.parametrize('dtype', (torch.bfloat16, torch.float32), ids=('bf16', 'fp32'))
 def test_nvfp4_writes_its_output_only(cuda_device, rows, hidden, dtype):
