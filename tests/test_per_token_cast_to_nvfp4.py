@@ -149,3 +149,24 @@ def test_cpu_tensors_are_refused():
     from tilekernels_b200 import quant
     with pytest.raises(AssertionError):
         quant.per_token_cast_to_nvfp4(torch.zeros((4, 64)), torch.ones(1))
+
+
+@pytest.mark.parametrize('rows,blocks', ((5, 1), (1, 1), (4, 3)))
+def test_other_casts_refuse_e4m3_scales(rows, blocks):
+    """One block per row, or transposed scales: unit stride along rows, which float32 and packed scales have in column-major
+    storage.  Read as float32, e4m3 bytes would be read four times as far as they reach."""
+    from tilekernels_b200 import quant
+    from tilekernels_b200.quant.common import get_cast_input_and_config
+    data = torch.zeros((rows, blocks * 8), dtype=torch.int8)
+    sf = torch.zeros((blocks, rows), dtype=torch.uint8).view(torch.float8_e4m3fn).T
+    assert sf.stride(0) == 1
+    for block in ((1, 16), (1, 32)):
+        with pytest.raises(AssertionError, match='scales'):
+            get_cast_input_and_config((data, sf), block)
+    with pytest.raises(AssertionError, match='scales'):
+        quant.per_token_cast((data, sf), 'e4m3', 16, (1, 16))
+    with pytest.raises(AssertionError, match='scales'):
+        quant.per_block_cast_lossless((data, sf), 'e4m3', (1, 16), (1, 32))
+    for dtype in (torch.bfloat16, torch.uint8):
+        with pytest.raises(AssertionError, match='scales'):
+            get_cast_input_and_config((data, torch.zeros((blocks, rows), dtype=dtype).T), (1, 32))

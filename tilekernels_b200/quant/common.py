@@ -85,6 +85,7 @@ def get_cast_input_and_config(
         config = CastInputConfig(torch_dtype=x.dtype, with_sf=True, sf_block=tuple(sf_block))
         assert isinstance(x, torch.Tensor) and isinstance(x_sf, torch.Tensor)
         assert x.dtype in (torch.float8_e4m3fn, torch.int8, torch.uint8)
+        assert x_sf.dtype in (torch.float32, torch.int32), 'scales are float32 or packed ue8m0 words (int32)'
         if x_sf.stride(0) == 1:
             config = replace(config, use_tma_aligned_col_major_sf=True)
             x_sf = x_sf.T
