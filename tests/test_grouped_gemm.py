@@ -169,6 +169,29 @@ def test_wgrad_of_small_weights(cuda_device, sizes, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('sizes,n,k', (((40, 0), 1032, 2056), ((300, 200), 2048, 1160), ((4100,), 128, 136)), ids=str)
+def test_accumulation_keeps_subnormals(cuda_device, sizes, n, k):
+    """An addition in fp32 as it is defined, in whole tiles and in products that a cluster shares: a subnormal is kept where nothing
+    is added to it, and counts where something is."""
+    from tilekernels_b200 import moe
+    start, end, used = segments(sizes)
+    s, e = int32(start, cuda_device), int32(end, cuda_device)
+    g = torch.zeros((used, -(-n // 8) * 8), dtype=torch.bfloat16, device=cuda_device)[:, :n]
+    x = torch.zeros((used, k), dtype=torch.bfloat16, device=cuda_device)
+    x[0] = 2.0 ** -63
+    tiny = torch.tensor([1e-40, -1e-40, 2.0 ** -149, 2.0 ** -126, 0.0, 3.0], device=cuda_device)
+    before = tiny[torch.arange(len(sizes) * n * k, device=cuda_device) % 6].view(len(sizes), n, k)
+    out = before.clone()
+    moe.grouped_gemm_wgrad(g, x, s, e, out=out, accumulate=True)
+    assert torch.equal(out.view(torch.int32), before.view(torch.int32))
+    g[0] = 2.0 ** -63   # every result of the first group is 2^-126
+    moe.grouped_gemm_wgrad(g, x, s, e, out=out, accumulate=True)
+    want = before.cpu().double()
+    want[0] += 2.0 ** -126   # (exact in fp32 but for 3.0, which stays)
+    assert torch.equal(out.cpu(), want.float())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('rows', (250, 1025, 9000))
 def test_wgrad_of_long_groups_keeps_its_precision(cuda_device, rows):
     """The tensor core's sum goes on in registers every 256 rows.  A step of 16 rows cuts off at most one unit (2^-23 of the

@@ -319,9 +319,29 @@ __device__ __forceinline__ void add_f32(float (&sum)[128], uint32_t taddr, uint3
     }
 }
 
+// Rows FROM .. FROM + N of a lane's column: what `out` holds plus the sum, N loads in flight.
+template <uint32_t FROM, uint32_t N>
+__device__ __forceinline__ void accumulate_rows(const float (&sum)[128], float*& o, int64_t stride, uint32_t rows) {
+    if (FROM >= rows) return;
+    const float* from = o;
+    float old[N];
+#pragma unroll
+    for (uint32_t q = 0; q < N; ++q) {
+        old[q] = 0.0f;
+        if (FROM + q < rows) asm volatile("ld.global.f32 %0, [%1];" : "=f"(old[q]) : "l"(from) : "memory");
+        from += stride;
+    }
+#pragma unroll
+    for (uint32_t q = 0; q < N; ++q) {
+        if (FROM + q < rows) asm volatile("st.global.f32 [%0], %1;" ::"l"(o), "f"(__fadd_rn(old[q], sum[FROM + q])) : "memory");
+        o += stride;
+    }
+}
+
 // A warp's 32 lanes hold 32 neighbouring columns, 128 bytes of a row, so every store is a whole line as it is.  (Shared memory
 // is what the products are short of: staged rows and TMA stores took 600 us where these took 540, 16 experts, 8192 rows,
-// 4096 x 7168.)  An accumulating call adds in L2, each element once.
+// 4096 x 7168.)  An accumulating call reads, adds and writes: each element has one owner.  Registers of sums that are stored take
+// later loads.  (Additions in L2 by red.global.add.f32 would flush subnormals of either side to zero.)
 __device__ __forceinline__ void store_f32(const GemmParams& p, const float (&sum)[128], float* o, uint32_t rows) {
     if (rows >= 128 && !p.accumulate) {
 #pragma unroll
@@ -329,15 +349,19 @@ __device__ __forceinline__ void store_f32(const GemmParams& p, const float (&sum
             asm volatile("st.global.L1::no_allocate.f32 [%0], %1;" ::"l"(o), "f"(sum[q]) : "memory");
             o += p.out_stride;
         }
-    } else {
+    } else if (!p.accumulate) {
 #pragma unroll
         for (uint32_t q = 0; q < 128; ++q) {
-            if (q < rows) {
-                if (p.accumulate) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(o), "f"(sum[q]) : "memory");
-                else *o = sum[q];
-            }
+            if (q < rows) *o = sum[q];
             o += p.out_stride;
         }
+    } else {
+        accumulate_rows<0, 8>(sum, o, p.out_stride, rows);
+        accumulate_rows<8, 16>(sum, o, p.out_stride, rows);
+        accumulate_rows<24, 16>(sum, o, p.out_stride, rows);
+        accumulate_rows<40, 24>(sum, o, p.out_stride, rows);
+        accumulate_rows<64, 32>(sum, o, p.out_stride, rows);
+        accumulate_rows<96, 32>(sum, o, p.out_stride, rows);
     }
 }
 
@@ -683,6 +707,18 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 const GemmTile tile = sched.tile(p, t);
                 if (tile.k_stages == 0 && p.accumulate) continue;
                 const uint32_t c = rw / 4 * 128, columns = tile.jn > c ? tile.jn - c : 0;  // the warp's 128 columns of the tile
+                if (!C::SPLIT && p.accumulate) {
+                    // What the sums are added to comes to L2 meanwhile; one lane per row, and its last column where a row's 128 bytes
+                    // end in another line (16 experts, 8192 rows, 4096 x 7168, accumulating: 1175 us without, 824 us so).
+                    const uint32_t iw = tile.i0 + rank * 128u + quarter * 32u, width = iw < p.i_size ? min(32u, p.i_size - iw) : 0;
+                    const float* row = static_cast<const float*>(p.out) + static_cast<int64_t>(tile.e) * p.out_group_stride +
+                                       static_cast<int64_t>(tile.j0 + c + lane) * p.out_stride + iw;
+                    for (uint32_t q = lane; width > 0 && q < min(columns, 128u); q += 32) {
+                        prefetch_l2(row);
+                        prefetch_l2(row + width - 1);
+                        row += 32 * p.out_stride;
+                    }
+                }
                 float sum[128];
 #pragma unroll
                 for (uint32_t q = 0; q < 128; ++q) sum[q] = 0.0f;

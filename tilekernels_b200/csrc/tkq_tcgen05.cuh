@@ -50,6 +50,8 @@ __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // Tile loads of a three-dimensional tensor; x * element size is a multiple of 16 bytes.  With CG = 2 the barrier may
 // belong to either CTA of the pair.
 template <int CG>
