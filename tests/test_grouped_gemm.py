@@ -209,6 +209,30 @@ def test_wgrad_of_long_groups_keeps_its_precision(cuda_device, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('sizes', ((300000,), (5, 20000, 0, 180000)), ids=str)
+def test_bf16_wgrad_of_very_long_groups(cuda_device, sizes):
+    """A sum of one sign over many rows, rounded to bf16: half a step of bf16, and before it what the sum itself is off by.  The tensor
+    core adds up 4096 rows at most, 256 steps of 16 rows that cut off at most one unit (2^-23) of the accumulator and one of each of
+    their products (2^-23 of the sum over one step, 1/256 of the sum); every addition in registers rounds by at most half a unit.
+    Left to the tensor core alone, 300000 rows came out 1.9e-3 of the result further off."""
+    from tilekernels_b200 import moe
+    n, k = 1152, 1152
+    start, end, used = segments(sizes, first=3)
+    gen = torch.Generator(cuda_device).manual_seed(used)
+    g = (torch.rand((used, n), generator=gen, device=cuda_device) + 0.5).to(torch.bfloat16)
+    x = (torch.rand((used, k), generator=gen, device=cuda_device) + 0.5).to(torch.bfloat16)
+    got = moe.grouped_gemm_wgrad(g, x, int32(start, cuda_device), int32(end, cuda_device), out_dtype=torch.bfloat16)
+    for i, (a, b) in enumerate(zip(start, end)):
+        want = torch.zeros((n, k), dtype=torch.float64, device=cuda_device)
+        for r in range(a, b, 1 << 15):
+            want += g[r:min(b, r + (1 << 15))].double().T @ x[r:min(b, r + (1 << 15))].double()
+        bound = (272 * 2.0 ** -23 + -(-sizes[i] // 4096) * 2.0 ** -24) * want
+        # half the distance of two bf16 numbers at `want`, or of the next binade where the sum may have reached it
+        half = torch.exp2(torch.floor(torch.log2((want + bound).clamp(min=2.0 ** -100))) - 8)
+        assert ((got[i].double() - want).abs() <= half + bound).all()
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences(cuda_device):
     """The product is linear in either operand, and with small integers every sum is exact, so differences of the forward
     product have to equal the gradients to the last bit."""

@@ -60,12 +60,13 @@ struct GemmParams {
     uint32_t wide_out;  // rows of out on 16-byte boundaries and i_size a multiple of 8
 };
 
-template <int KIND_, int CG_, int NMAX_, bool WGRAD_, bool A_MN_, bool SPLIT_ = false, bool F32_ = false>
+// F32: the weight gradient's sums go on in registers (see add_f32).  LONG: seldom, and the results are bf16.
+template <int KIND_, int CG_, int NMAX_, bool WGRAD_, bool A_MN_, bool SPLIT_ = false, bool F32_ = false, bool LONG_ = false>
 struct GemmConfig {
     static constexpr int KIND = KIND_, CG = CG_, NMAX = NMAX_;
-    static constexpr bool WGRAD = WGRAD_, A_MN = A_MN_, SCALED = KIND_ != kKindBf16, SPLIT = SPLIT_, F32 = F32_;
-    // fp32 results: stages whose products the tensor core adds up before the sum goes on in registers (see add_f32)
-    static constexpr uint32_t kChunk = F32 ? 4 : 1u << 30;
+    static constexpr bool WGRAD = WGRAD_, A_MN = A_MN_, SCALED = KIND_ != kKindBf16, SPLIT = SPLIT_, F32 = F32_, LONG = LONG_;
+    // stages whose products the tensor core adds up before the sum goes on in registers
+    static constexpr uint32_t kChunk = !F32 ? 1u << 30 : LONG ? 64 : 4;
     // A stage holds kSub blocks of 128 bytes along K.  Waiting for a stage and handing it back costs the issuing warp some
     // 200 cycles: two thirds of a block's products in 4 or 8 bits (448 cycles at N = 224), which therefore come in pairs
     static constexpr uint32_t kSub = SCALED ? 2 : 1;
@@ -301,11 +302,12 @@ __device__ __forceinline__ void store_bf16(const GemmParams& p, const GemmTile& 
 __device__ __forceinline__ uint32_t as_bits(uint32_t x) { return x; }
 __device__ __forceinline__ uint32_t as_bits(float x) { return __float_as_uint(x); }
 
-// fp32 results of the weight gradient.  The tensor core cuts off what an addition to its accumulator shifts out instead of
-// rounding, so a long sum drifts towards zero by about 2.3e-8 of itself per step of 16 rows (groups of some 900 rows: 1.3e-6
-// off).  Every 16 steps its sum is therefore added to one in registers, with rounding: eight warps hold 128 columns of the
-// tile each, and the accumulators take turns, so that this goes on beside the products (16 experts, 8192 rows, 4096 x 7168:
-// 2.4e-7 off and 560 us; 4.8e-7 and 552 us with 32 steps; 1.3e-6 and 540 us without).
+// Sums of the weight gradient in registers.  The tensor core cuts off what an addition to its accumulator shifts out instead of
+// rounding, so a long sum drifts towards zero, by less than one unit (2^-23 of itself) per step of 16 rows; over groups of some
+// 900 rows 1.3e-6 was measured, over 300000 rows of one sign 1.9e-3.  Every kChunk stages its sum is therefore added to one in
+// registers, with rounding: eight warps hold 128 columns of the tile each, and the accumulators take turns, so that this goes on
+// beside the products.  fp32 results: every 16 steps (16 experts, 8192 rows, 4096 x 7168: 2.4e-7 off and 560 us; 4.8e-7 and 552 us
+// with 32 steps; 1.3e-6 and 540 us without).  bf16 results: every 256 steps, 2^-15 at most (half a step of bf16 is 2^-9 or more).
 __device__ __forceinline__ void add_f32(float (&sum)[128], uint32_t taddr, uint32_t columns) {
 #pragma unroll
     for (uint32_t g = 0; g < 8; ++g) {
@@ -362,6 +364,15 @@ __device__ __forceinline__ void store_f32(const GemmParams& p, const float (&sum
         accumulate_rows<40, 24>(sum, o, p.out_stride, rows);
         accumulate_rows<64, 32>(sum, o, p.out_stride, rows);
         accumulate_rows<96, 32>(sum, o, p.out_stride, rows);
+    }
+}
+
+// bf16: 64 bytes of a row per warp.
+__device__ __forceinline__ void store_long_bf16(const GemmParams& p, const float (&sum)[128], __nv_bfloat16* o, uint32_t rows) {
+#pragma unroll
+    for (uint32_t q = 0; q < 128; ++q) {
+        if (q < rows) *o = __float2bfloat16_rn(sum[q]);
+        o += p.out_stride;
     }
 }
 
@@ -736,9 +747,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 const uint32_t i = tile.i0 + rank * 128u + quarter * 32u + lane;
                 if constexpr (C::SPLIT) {
                     if (ok && c < C::NMAX) hand_over<C>(sum, 0, quarter * 32 + lane, p.split, part, partial);
-                } else if (ok && i < p.i_size)
-                    store_f32(p, sum, static_cast<float*>(p.out) + static_cast<int64_t>(tile.e) * p.out_group_stride +
-                                          static_cast<int64_t>(tile.j0 + c) * p.out_stride + i, columns);
+                } else if (ok && i < p.i_size) {
+                    const int64_t at = static_cast<int64_t>(tile.e) * p.out_group_stride + static_cast<int64_t>(tile.j0 + c) * p.out_stride + i;
+                    if constexpr (C::LONG) store_long_bf16(p, sum, static_cast<__nv_bfloat16*>(p.out) + at, columns);
+                    else store_f32(p, sum, static_cast<float*>(p.out) + at, columns);
+                }
             }
         }
         if (!C::WGRAD && p.zero_gaps) {
