@@ -280,12 +280,13 @@ extern "C" int tkq_grouped_gemm_wgrad(const tkq_grouped_gemm_wgrad_args* args, v
     p.split = split_of(num_experts * ((n + 127) / 128) * ((k + 127) / 128), num_rows / num_experts / 64, 8);
     if (p.split > 1) {
         p.out_bf16 = out_dtype == TKQ_DT_BF16;
-        return launch_gemm<GemmConfig<kKindBf16, 1, 128, true, true, true, true>>(a, b, p, "grouped_gemm_wgrad", s);
+        return launch_gemm<GemmConfig<kKindBf16, 1, 128, true, true, true, kSumsF32>>(a, b, p, "grouped_gemm_wgrad", s);
     }
-    if (out_dtype == TKQ_DT_FP32) return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true, false, true>>(a, b, p, "grouped_gemm_wgrad", s);
+    if (p.accumulate) return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true, false, kSumsAccumulate>>(a, b, p, "grouped_gemm_wgrad", s);
+    if (out_dtype == TKQ_DT_FP32) return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true, false, kSumsF32>>(a, b, p, "grouped_gemm_wgrad", s);
     // bf16: up to 16384 rows what the tensor core cuts off (2^-23 per 16 rows, together 2^-13) is little beside the rounding to bf16.
     // Longer calls have their sums go on in registers every 4096 rows: groups can be long, and their bounds are known on the device
     // only.  (Without against with, 4096 x 7168: 16 experts of 1024 rows 685, 703 us; one of 32768 rows 1395, 1407.)
-    if (num_rows > 16384) return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true, false, true, true>>(a, b, p, "grouped_gemm_wgrad", s);
+    if (num_rows > 16384) return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true, false, kSumsBf16>>(a, b, p, "grouped_gemm_wgrad", s);
     return launch_gemm<GemmConfig<kKindBf16, 2, 256, true, true>>(a, b, p, "grouped_gemm_wgrad", s);
 }

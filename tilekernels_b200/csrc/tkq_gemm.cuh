@@ -60,13 +60,17 @@ struct GemmParams {
     uint32_t wide_out;  // rows of out on 16-byte boundaries and i_size a multiple of 8
 };
 
-// F32: the weight gradient's sums go on in registers (see add_f32).  LONG: seldom, and the results are bf16.
-template <int KIND_, int CG_, int NMAX_, bool WGRAD_, bool A_MN_, bool SPLIT_ = false, bool F32_ = false, bool LONG_ = false>
+// Where the weight gradient's sums go on in registers (see add_f32), and what becomes of them
+constexpr int kSumsNone = 0, kSumsF32 = 1, kSumsAccumulate = 2, kSumsBf16 = 3;
+
+template <int KIND_, int CG_, int NMAX_, bool WGRAD_, bool A_MN_, bool SPLIT_ = false, int SUMS_ = kSumsNone>
 struct GemmConfig {
     static constexpr int KIND = KIND_, CG = CG_, NMAX = NMAX_;
-    static constexpr bool WGRAD = WGRAD_, A_MN = A_MN_, SCALED = KIND_ != kKindBf16, SPLIT = SPLIT_, F32 = F32_, LONG = LONG_;
+    static constexpr bool WGRAD = WGRAD_, A_MN = A_MN_, SCALED = KIND_ != kKindBf16, SPLIT = SPLIT_;
+    static constexpr int SUMS = SUMS_;
+    static constexpr bool F32 = SUMS != kSumsNone;
     // stages whose products the tensor core adds up before the sum goes on in registers
-    static constexpr uint32_t kChunk = !F32 ? 1u << 30 : LONG ? 64 : 4;
+    static constexpr uint32_t kChunk = !F32 ? 1u << 30 : SUMS == kSumsBf16 ? 64 : 4;
     // A stage holds kSub blocks of 128 bytes along K.  Waiting for a stage and handing it back costs the issuing warp some
     // 200 cycles: two thirds of a block's products in 4 or 8 bits (448 cycles at N = 224), which therefore come in pairs
     static constexpr uint32_t kSub = SCALED ? 2 : 1;
@@ -342,29 +346,32 @@ __device__ __forceinline__ void accumulate_rows(const float (&sum)[128], float*&
 
 // A warp's 32 lanes hold 32 neighbouring columns, 128 bytes of a row, so every store is a whole line as it is.  (Shared memory
 // is what the products are short of: staged rows and TMA stores took 600 us where these took 540, 16 experts, 8192 rows,
-// 4096 x 7168.)  An accumulating call reads, adds and writes: each element has one owner.  Registers of sums that are stored take
-// later loads.  (Additions in L2 by red.global.add.f32 would flush subnormals of either side to zero.)
+// 4096 x 7168.)
 __device__ __forceinline__ void store_f32(const GemmParams& p, const float (&sum)[128], float* o, uint32_t rows) {
-    if (rows >= 128 && !p.accumulate) {
+    if (rows >= 128) {
 #pragma unroll
         for (uint32_t q = 0; q < 128; ++q) {
             asm volatile("st.global.L1::no_allocate.f32 [%0], %1;" ::"l"(o), "f"(sum[q]) : "memory");
             o += p.out_stride;
         }
-    } else if (!p.accumulate) {
+    } else {
 #pragma unroll
         for (uint32_t q = 0; q < 128; ++q) {
             if (q < rows) *o = sum[q];
             o += p.out_stride;
         }
-    } else {
-        accumulate_rows<0, 8>(sum, o, p.out_stride, rows);
-        accumulate_rows<8, 16>(sum, o, p.out_stride, rows);
-        accumulate_rows<24, 16>(sum, o, p.out_stride, rows);
-        accumulate_rows<40, 24>(sum, o, p.out_stride, rows);
-        accumulate_rows<64, 32>(sum, o, p.out_stride, rows);
-        accumulate_rows<96, 32>(sum, o, p.out_stride, rows);
     }
+}
+
+// An accumulating call reads, adds and writes: each element has one owner.  Registers of sums that are stored take later loads.
+// (Additions in L2 by red.global.add.f32 would flush subnormals of either side to zero.)
+__device__ __forceinline__ void accumulate_f32(const GemmParams& p, const float (&sum)[128], float* o, uint32_t rows) {
+    accumulate_rows<0, 8>(sum, o, p.out_stride, rows);
+    accumulate_rows<8, 16>(sum, o, p.out_stride, rows);
+    accumulate_rows<24, 16>(sum, o, p.out_stride, rows);
+    accumulate_rows<40, 24>(sum, o, p.out_stride, rows);
+    accumulate_rows<64, 32>(sum, o, p.out_stride, rows);
+    accumulate_rows<96, 32>(sum, o, p.out_stride, rows);
 }
 
 // bf16: 64 bytes of a row per warp.
@@ -718,7 +725,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 const GemmTile tile = sched.tile(p, t);
                 if (tile.k_stages == 0 && p.accumulate) continue;
                 const uint32_t c = rw / 4 * 128, columns = tile.jn > c ? tile.jn - c : 0;  // the warp's 128 columns of the tile
-                if (!C::SPLIT && p.accumulate) {
+                if constexpr (C::SUMS == kSumsAccumulate && !C::SPLIT) {
                     // What the sums are added to comes to L2 meanwhile; one lane per row, and its last column where a row's 128 bytes
                     // end in another line (16 experts, 8192 rows, 4096 x 7168, accumulating: 1175 us without, 824 us so).
                     const uint32_t iw = tile.i0 + rank * 128u + quarter * 32u, width = iw < p.i_size ? min(32u, p.i_size - iw) : 0;
@@ -749,7 +756,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                     if (ok && c < C::NMAX) hand_over<C>(sum, 0, quarter * 32 + lane, p.split, part, partial);
                 } else if (ok && i < p.i_size) {
                     const int64_t at = static_cast<int64_t>(tile.e) * p.out_group_stride + static_cast<int64_t>(tile.j0 + c) * p.out_stride + i;
-                    if constexpr (C::LONG) store_long_bf16(p, sum, static_cast<__nv_bfloat16*>(p.out) + at, columns);
+                    if constexpr (C::SUMS == kSumsBf16) store_long_bf16(p, sum, static_cast<__nv_bfloat16*>(p.out) + at, columns);
+                    else if constexpr (C::SUMS == kSumsAccumulate) accumulate_f32(p, sum, static_cast<float*>(p.out) + at, columns);
                     else store_f32(p, sum, static_cast<float*>(p.out) + at, columns);
                 }
             }
@@ -775,7 +783,6 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             const GemmTile tile = sched.tile(p, t);
             const uint32_t a = acc_it & 1u;
             const bool have = tile.k_stages > 0;
-            if (!have && p.accumulate) continue;
             if (have) {
                 const bool ok = wait(bar(&acc_full[a]), (acc_it >> 1) & 1u);
                 if (!__all_sync(kFullMask, ok)) break;
