@@ -209,6 +209,24 @@ def test_wgrad_of_long_groups_keeps_its_precision(cuda_device, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('rows,n,k', ((9000, 2048, 2048), (80000, 136, 264)), ids=('whole', 'split'))
+def test_wgrad_sums_of_one_sign_do_not_drift(cuda_device, rows, n, k):
+    """What the tensor core cuts off has one sign, so it shows in the mean over all results.  Step t of the 16 between two additions
+    in registers cuts off at most one unit (2^-23) of t / 16 of their sum: 8.5 units in all, where a sum left to the tensor core
+    over 560 steps or more would lose some 280 (half a unit per step on average; 265 of 2^-23 were measured).  Additions in registers round
+    either way; what is left of them in the mean is granted as much again."""
+    from tilekernels_b200 import moe
+    gen = torch.Generator(cuda_device).manual_seed(rows)
+    g = (torch.rand((rows, n), generator=gen, device=cuda_device) + 0.5).to(torch.bfloat16)
+    x = (torch.rand((rows, k), generator=gen, device=cuda_device) + 0.5).to(torch.bfloat16)
+    before = torch.zeros((1, n, k), device=cuda_device)
+    bounds = int32([0], cuda_device), int32([rows], cuda_device)
+    want = g.double().T @ x.double()
+    for got in (moe.grouped_gemm_wgrad(g, x, *bounds)[0], moe.grouped_gemm_wgrad(g, x, *bounds, out=before, accumulate=True)[0]):
+        assert abs(((got.double() - want) / want).mean().item()) <= 17 * 2.0 ** -23
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('sizes', ((300000,), (5, 20000, 0, 180000)), ids=str)
 def test_bf16_wgrad_of_very_long_groups(cuda_device, sizes):
     """A sum of one sign over many rows, rounded to bf16: half a step of bf16, and before it what the sum itself is off by.  The tensor
