@@ -59,6 +59,27 @@ def test_argument_checks_of_the_products(lib):
     assert b'grouped_gemm_wgrad' in lib.tkq_last_error_string()
 
 
+def test_expanded_operands_are_refused_by_name(lib):
+    """An axis of stride 0 is no matter of 16-byte boundaries."""
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    from tilekernels_b200 import _lib
+
+    def refused(rc, what):
+        return rc == -2 and what in lib.tkq_last_error_string() and b'stride 0' in lib.tkq_last_error_string()
+
+    for x_row, w_expert, w_row in ((0, 1024, 128), (128, 0, 128), (128, 1024, 0)):
+        rc = lib.tkq_block_scaled_gemm(_lib.BLOCK_SCALED_GEMM_ARGS.pack(p, x_row, p, 1, 4, 1, 128, p, w_expert, w_row, p, 0, 1, 8, 1, 128, 0, 0, p, p, 2, 4, 8, 128,
+                                                                        0, 0, p, 8, 0), None)
+        assert refused(rc, b'block_scaled_gemm')
+        for transpose in (0, 1):
+            assert refused(lib.tkq_grouped_gemm(_lib.GROUPED_GEMM_ARGS.pack(p, x_row, p, w_expert, w_row, transpose, p, p, 2, 4, 64, 64, p, 64, 0), None),
+                           b'grouped_gemm')
+    for g_row, x_row in ((0, 64), (64, 0)):
+        rc = lib.tkq_grouped_gemm_wgrad(_lib.GROUPED_GEMM_WGRAD_ARGS.pack(p, g_row, p, x_row, p, p, 2, 4, 64, 64, 1, p, 0), None)
+        assert refused(rc, b'grouped_gemm_wgrad')
+
+
 def test_argument_checks_of_the_nvfp4_entry_points(lib):
     buf = (ctypes.c_char * 4096)()
     p16 = (ctypes.addressof(buf) + 15) // 16 * 16

@@ -39,12 +39,14 @@ static int encode(CUtensorMap* map, const Operand& o, uint32_t box_inner, uint32
     return 0;
 }
 
-// Strides a tensor map accepts: multiples of 16 bytes.  The stride of an axis of length one is never used, so any stands in.
-static bool fix_strides(Operand& o) {
+// Strides a tensor map accepts: positive multiples of 16 bytes.  The stride of an axis of length one is never used, so any stands in.
+static int fix_strides(Operand& o, const char* expanded, const char* unaligned) {
     const int64_t tight = (o.inner * (o.bf16 ? 2 : 1) + 15) / 16 * 16;
     if (o.rows == 1) o.row_bytes = tight;
     if (o.groups == 1) o.group_bytes = o.row_bytes * o.rows;
-    return o.row_bytes % 16 == 0 && o.group_bytes % 16 == 0 && o.row_bytes > 0 && o.group_bytes > 0 && aligned16(o.base);
+    if (o.row_bytes <= 0 || o.group_bytes <= 0) return set_error(TKQ_E_UNSUPPORTED, expanded);
+    if (o.row_bytes % 16 || o.group_bytes % 16 || !aligned16(o.base)) return set_error(TKQ_E_ALIGNMENT, unaligned);
+    return 0;
 }
 
 template <class C>
@@ -174,9 +176,12 @@ extern "C" int tkq_block_scaled_gemm(const tkq_block_scaled_gemm_args* args, voi
         return set_error(TKQ_E_ALIGNMENT, "block_scaled_gemm: strides of packed e2m1 data are even");
     Operand a{w, k / per_byte, n, num_experts, w_row_stride / per_byte, w_expert_stride / per_byte, false};
     Operand b{x, k / per_byte, num_rows, 1, x_row_stride / per_byte, 0, false};
-    if (!fix_strides(a) || !fix_strides(b) || (reinterpret_cast<uintptr_t>(x_sf) & 3u) || (reinterpret_cast<uintptr_t>(w_sf) & 3u) ||
-        (reinterpret_cast<uintptr_t>(out) & 1u))
-        return set_error(TKQ_E_ALIGNMENT, "block_scaled_gemm: data rows on 16-byte boundaries, scales on 4-byte boundaries");
+    constexpr const char* expanded = "block_scaled_gemm: data whose rows or matrices have stride 0 (an expanded tensor); make it contiguous";
+    constexpr const char* unaligned = "block_scaled_gemm: data rows on 16-byte boundaries, scales on 4-byte boundaries";
+    if (int rc = fix_strides(a, expanded, unaligned)) return rc;
+    if (int rc = fix_strides(b, expanded, unaligned)) return rc;
+    if ((reinterpret_cast<uintptr_t>(x_sf) & 3u) || (reinterpret_cast<uintptr_t>(w_sf) & 3u) || (reinterpret_cast<uintptr_t>(out) & 1u))
+        return set_error(TKQ_E_ALIGNMENT, unaligned);
     GemmParams p{};
     p.start = expert_start;
     p.end = expert_end;
@@ -223,8 +228,11 @@ extern "C" int tkq_grouped_gemm(const tkq_grouped_gemm_args* args, void* stream)
         return set_error(TKQ_E_BAD_ARG, "grouped_gemm: null pointer");
     Operand a{w, transpose_w ? n : k, transpose_w ? k : n, num_experts, w_row_stride * 2, w_expert_stride * 2, true};
     Operand b{x, k, num_rows, 1, x_row_stride * 2, 0, true};
-    if (!fix_strides(a) || !fix_strides(b) || (reinterpret_cast<uintptr_t>(out) & 1u))
-        return set_error(TKQ_E_ALIGNMENT, "grouped_gemm: rows of x and w on 16-byte boundaries");
+    constexpr const char* expanded = "grouped_gemm: rows or matrices of stride 0 (an expanded tensor); make it contiguous";
+    constexpr const char* unaligned = "grouped_gemm: rows of x and w on 16-byte boundaries";
+    if (int rc = fix_strides(a, expanded, unaligned)) return rc;
+    if (int rc = fix_strides(b, expanded, unaligned)) return rc;
+    if (reinterpret_cast<uintptr_t>(out) & 1u) return set_error(TKQ_E_ALIGNMENT, unaligned);
     GemmParams p{};
     p.start = expert_start;
     p.end = expert_end;
@@ -260,8 +268,11 @@ extern "C" int tkq_grouped_gemm_wgrad(const tkq_grouped_gemm_wgrad_args* args, v
     }
     Operand a{x, k, num_rows, 1, x_row_stride * 2, 0, true};
     Operand b{grad, n, num_rows, 1, grad_row_stride * 2, 0, true};
-    if (!fix_strides(a) || !fix_strides(b) || (reinterpret_cast<uintptr_t>(out) & (out_dtype == TKQ_DT_FP32 ? 3u : 1u)))
-        return set_error(TKQ_E_ALIGNMENT, "grouped_gemm_wgrad: rows of grad and x on 16-byte boundaries");
+    constexpr const char* expanded = "grouped_gemm_wgrad: rows of stride 0 (an expanded tensor); make it contiguous";
+    constexpr const char* unaligned = "grouped_gemm_wgrad: rows of grad and x on 16-byte boundaries";
+    if (int rc = fix_strides(a, expanded, unaligned)) return rc;
+    if (int rc = fix_strides(b, expanded, unaligned)) return rc;
+    if (reinterpret_cast<uintptr_t>(out) & (out_dtype == TKQ_DT_FP32 ? 3u : 1u)) return set_error(TKQ_E_ALIGNMENT, unaligned);
     GemmParams p{};
     p.start = expert_start;
     p.end = expert_end;
