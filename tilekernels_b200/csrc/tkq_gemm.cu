@@ -112,18 +112,24 @@ static bool launch_split(const Operand& a, const Operand& b, GemmParams p, const
     return true;
 }
 
-// Tile variant by the mean number of rows per group.  Measured (us; 32 groups, 4096 x 7168, MXFP4 and bf16):
-//   mean rows          20          34          64         100         200
-//   128 x 32        83, -     105, 372    146, 540    198, 746   358, 1394
-//   128 x 128       85, -      87, 287     93, 306    106, 361   148, 510
-//   pair x 224/256  88, -      90, 288     92, 294     97, 315   124, 406
+// Tile variant by the mean number of rows per group (over all rows: which of them belong to a group, and how evenly, is known on
+// the device only).  Measured (us; 32 groups, 4096 x 7168, MXFP4 and bf16, groups of one size):
+//   mean rows           4          20          32          34          64         100         200
+//   128 x 32       80, 271     83, 275     84, 277    120, 427    146, 540    198, 746   358, 1394
+//   128 x 128      83, 284     85, 288     86, 289     88, 292     93, 306    106, 361    148, 510
+//   pair x 224/256 87, 289     89, 293     89, 295     90, 297     92, 294     97, 315    124, 406
+// Groups of skewed sizes (the longest three times the mean) reach the second tile, and read their weight again, at a smaller mean:
+//   mean rows           4           8          16          20          24          32
+//   128 x 32       60, 200     71, 238     81, 275     83, 274     90, 309    100, 345
+//   128 x 128      63, 209     74, 247     78, 262     81, 271     83, 280     84, 282
+// so several groups take 128 x 32 up to a mean of 16, one group while its rows are one such tile.
 // One group whose smaller tiles all run at once uses more SMs with them (200 rows of MXFP4: 13.0 against 16.3 us for the
 // pair, 256 of FP8: 20.8 against 22.3).
 template <int KIND, int NMID, int NLARGE, bool A_MN>
 static int launch_rows(const Operand& a, const Operand& b, const GemmParams& p, const char* what, cudaStream_t stream) {
     const int64_t mean = p.rows / p.groups;
     int rc;
-    if (mean <= 32) {
+    if (mean <= (p.groups == 1 ? 32 : 16)) {
         if (launch_split<KIND, 32, A_MN>(a, b, p, what, stream, &rc)) return rc;
         return launch_gemm<GemmConfig<KIND, 1, 32, false, A_MN>>(a, b, p, what, stream);
     }
