@@ -351,7 +351,9 @@ int tkq_cast_back_nvfp4(const void* x, const void* sf, const float* tensor_scale
 /*
  * Products of quantized matrices: out[r, i] = alpha_e * sum_k x[r, k] * w[e, i, k] in fp32, rounded once to bf16, for the
  * rows r of group e, expert_start[e] <= r < expert_end[e].  The operands stay in their 8- or 4-bit form on the way to the
- * tensor core, which applies the block scales.  No counterpart in the reference.
+ * tensor core, which applies the block scales.  Its fp32 sums cut off what an addition shifts out instead of rounding: 2^-23
+ * of the sum at most per step of 32 (e4m3), 64 (e2m1) or, in the bf16 products below, 16 values.  No counterpart in the
+ * reference.
  *
  *   x                [num_rows, k] and  w [num_experts, n, k]: e4m3 bytes, or e2m1 pairs (strides count values)
  *   x_sf, w_sf       four scale bytes per 32-bit word along k: word q of row block m at m * row_stride + q * k_stride
@@ -362,7 +364,8 @@ int tkq_cast_back_nvfp4(const void* x, const void* sf, const float* tensor_scale
  *   fmt, sf_fmt      TKQ_FMT_E4M3 or TKQ_FMT_E2M1; TKQ_SFMT_UE8M0, or TKQ_SFMT_E4M3 with e2m1
  *   expert_start/end int32[num_experts], ascending and disjoint; values outside [0, num_rows] are clamped, and a group has
  *                    no rows before the end of an earlier one.  Both NULL with num_experts = 1: one group of all rows
- *   k                multiple of 32 (e4m3) or 64 (e2m1); data rows start on 16-byte boundaries
+ *   k                multiple of 32 (e4m3) or 64 (e2m1); data rows start on 16-byte boundaries; axes of the data that are longer
+ *                    than one have strides above 0 (TKQ_E_UNSUPPORTED)
  *   alpha            NULL or fp32, alpha[e * alpha_stride]
  *   out              bf16 [num_rows, out_row_stride]; rows of no group are left alone, or cleared with TKQ_ZERO_GAPS
  */
@@ -389,7 +392,7 @@ int tkq_block_scaled_gemm(const tkq_block_scaled_gemm_args* args, void* stream);
 
 /*
  * bf16 products grouped by expert: out[r, i] = sum_k x[r, k] * w[e, i, k], or with transpose_w (the gradient of the rows)
- * out[r, i] = sum_k x[r, k] * w[e, k, i], for the rows r of group e; fp32 sums, one rounding to bf16.  Groups, rows of no
+ * out[r, i] = sum_k x[r, k] * w[e, k, i], for the rows r of group e; fp32 sums as above, one rounding to bf16.  Groups, rows of no
  * group and alignment as in tkq_block_scaled_gemm.  No counterpart in the reference.
  *
  *   x    [num_rows, k] bf16;  w  [num_experts, n, k], with transpose_w [num_experts, k, n]; rows on 16-byte boundaries
@@ -411,7 +414,8 @@ int tkq_grouped_gemm(const tkq_grouped_gemm_args* args, void* stream);
 /*
  * Gradient of each expert's weight: out[e, j, i] (+)= sum over the rows r of group e of grad[r, j] * x[r, i], fp32 sums.
  * A group without rows gives zeros (with TKQ_ACCUMULATE: leaves its part alone).  Rows of no group are not read into any
- * sum, whatever they hold.  No counterpart in the reference.
+ * sum, whatever they hold.  The tensor core adds up 256 rows at a time for fp32 results and up to 16384 for bf16; longer
+ * sums go on as rounded fp32 additions, and TKQ_ACCUMULATE is one such addition.  No counterpart in the reference.
  *
  *   grad  [num_rows, n] bf16;  x  [num_rows, k] bf16; rows on 16-byte boundaries
  *   out   [num_experts, n, k] contiguous, bf16 or fp32 (out_dtype); TKQ_ACCUMULATE needs fp32

@@ -294,6 +294,7 @@ extern "C" int tkq_grouped_gemm_wgrad(const tkq_grouped_gemm_wgrad_args* args, v
     // Small results whose 128 x 128 tiles leave SMs idle: the rows of a group are split over a cluster.  Whole (pairs on 256 x
     // 256) against split: 20000 rows, 128 x 128: 102, 22 us; 4096 rows, 512 x 512: 27.5, 14.5; 8 experts, 16000 rows, 256 x 512:
     // 25.5, 21.6.  Parts of five or six stages gained nothing (700 rows, 512 x 512: 10.6, 10.9), so a part has at least eight.
+    // The mean decides here too: one long group among empty ones is not split.
     p.split = split_of(num_experts * ((n + 127) / 128) * ((k + 127) / 128), num_rows / num_experts / 64, 8);
     if (p.split > 1) {
         p.out_bf16 = out_dtype == TKQ_DT_BF16;

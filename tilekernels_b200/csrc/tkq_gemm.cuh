@@ -606,8 +606,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                         const uint32_t sfa = tmem + C::kSfBase + h % C::kSfSets * C::kSfCols, sfb = sfa + 4 * C::kWords;
                         uint32_t id0 = idesc;
                         if constexpr (C::SCALED) {
-                            // The copies go over the scales of an earlier block.  Copies and products of one thread run in the order of
-                            // their issue (they share a pipe), so nothing has to be waited for.
+                            // The copies go over the scales of an earlier block, whose products may still be under way.  Nothing is waited
+                            // for: PTX promises that a product sees the copies issued before it, and the hardware has been seen to keep
+                            // the order of issue the other way too, for which there is no such promise (test_many_waves compares products
+                            // whose scales differ from block to block).
                             const uint64_t dfa = desc_sf + now * ((C::kSub * (C::kSfaBytes + C::kSfbBytes)) >> 4);
                             const uint64_t dfb = dfa + ((C::kSub * C::kSfaBytes) >> 4);
                             const uint32_t ha = C::KIND == kKindMxf8 && p.sfa.k_shift ? 0 : h, hb = C::KIND == kKindMxf8 && p.sfb.k_shift ? 0 : h;
@@ -727,7 +729,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
                 const uint32_t c = rw / 4 * 128, columns = tile.jn > c ? tile.jn - c : 0;  // the warp's 128 columns of the tile
                 if constexpr (C::SUMS == kSumsAccumulate && !C::SPLIT) {
                     // What the sums are added to comes to L2 meanwhile; one lane per row, and its last column where a row's 128 bytes
-                    // end in another line (16 experts, 8192 rows, 4096 x 7168, accumulating: 1175 us without, 824 us so).
+                    // end in another line (16 experts, 8192 rows, 4096 x 7168, accumulating: 1175 us without, 826 us so).
                     const uint32_t iw = tile.i0 + rank * 128u + quarter * 32u, width = iw < p.i_size ? min(32u, p.i_size - iw) : 0;
                     const float* row = static_cast<const float*>(p.out) + static_cast<int64_t>(tile.e) * p.out_group_stride +
                                        static_cast<int64_t>(tile.j0 + c + lane) * p.out_stride + iw;

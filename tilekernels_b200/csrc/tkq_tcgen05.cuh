@@ -31,8 +31,10 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // Arrival at a barrier of any CTA of the cluster (address from map_to_rank).  What it announces is shared or tensor memory
-// of the arriving thread's own SM, ordered by a proxy or tcgen05 fence before it.  With .release.cluster the same arrival
-// waits for the thread's global loads and costs about a microsecond (16384 x 4096 x 7168 MXFP4: 511 us with it, 377 us without).
+// of the arriving thread's own SM, ordered by a proxy or tcgen05 fence before it.  Its scope is the default one, the CTA; with
+// .release.cluster the same arrival waits for the thread's global loads and costs about a microsecond (16384 x 4096 x 7168 MXFP4:
+// 511 us with it, 377 us without).  So for the other CTA of a pair the order rests on those fences and on how the hardware carries
+// them out, which PTX's memory model does not spell out for this scope; test_many_waves compares every result that depends on it.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }

@@ -96,9 +96,10 @@ def block_scaled_gemm(
     alpha: Optional[torch.Tensor] = None,
     out: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    """alpha * a @ b.T for two quantized matrices, in bfloat16 (one rounding of the fp32 sums).
+    """alpha * a @ b.T for two quantized matrices, in bfloat16.
 
-    The data reach the tensor core in their 8- or 4-bit form; the block scales are applied there.
+    The data reach the tensor core in their 8- or 4-bit form; the block scales are applied there.  Its fp32 sums cut off what an
+    addition shifts out (2^-23 of the sum at most per 32 values of k in FP8, 64 in FP4) and are rounded once to bfloat16.
 
     Args:
         a: (data, scales) of (m, k) values, b: of (n, k).  Both in one of the forms
@@ -106,7 +107,7 @@ def block_scaled_gemm(
             return them with use_packed_ue8m0;
             int8 data (two FP4 per byte) with packed ue8m0 scales per 32 values;
             int8 data with float8_e4m3fn scales per 16 values (per_token_cast_to_nvfp4).
-            k is a multiple of 32 (FP8) or 64 (FP4); rows of the data start on 16-byte boundaries.
+            k is a multiple of 32 (FP8) or 64 (FP4); rows of the data start on 16-byte boundaries and are not expanded.
         a_block_size, b_block_size: (rows, values) per scale; rows 1, 32 or 128.
         alpha: optional fp32 tensor of one element, e.g. the product of the tensor scales of two NVFP4 operands.
         out: optional (m, n) bfloat16 destination with unit column stride.
