@@ -93,6 +93,33 @@ def test_split_weight_gradients_write_their_output_only(cuda_device, n, k, dtype
     check_values(out, ((0, 17), (4000, 5000)))
 
 
+@pytest.mark.parametrize('mode', ('bf16', 'fp32', 'accumulate'))
+@pytest.mark.parametrize('n,k', ((1290, 1165), (1, 9500), (2049, 600)))
+def test_whole_weight_gradients_write_their_output_only(cuda_device, mode, n, k):
+    """Weights whose tiles fill the SMs, so that no group is split, in a call of more than 16384 rows; rows of no group hold NaN."""
+    from tilekernels_b200 import moe
+    gen = torch.Generator(cuda_device).manual_seed(n * k)
+    rows, bounds = 16500, ((2, 4200), (4200, 4200), (4207, 16497))
+    g = torch.randn((rows, -(-n // 8) * 8), generator=gen, device=cuda_device).to(torch.bfloat16)[:, :n]
+    x = torch.randn((rows, -(-k // 8) * 8), generator=gen, device=cuda_device).to(torch.bfloat16)[:, :k]
+    for a, b in ((0, 2), (4200, 4207), (16497, rows)):
+        g[a:b] = float('nan')
+        x[a:b] = float('inf')
+    s, e = (int32(list(v), cuda_device) for v in zip(*bounds))
+    dtype = torch.bfloat16 if mode == 'bf16' else torch.float32
+    out, check = _guarded((3, n, k), dtype, cuda_device)
+    if mode == 'accumulate':
+        out.zero_()
+    moe.grouped_gemm_wgrad(g, x, s, e, out_dtype=dtype, out=out, accumulate=mode == 'accumulate')
+    check()
+    for i, (a, b) in enumerate(bounds):
+        a64, b64 = g[a:b].double(), x[a:b].double()
+        want, bound = a64.T @ b64, (b - a) * 2.0 ** -23 * (a64.abs().T @ b64.abs())
+        if mode == 'bf16':
+            bound += 2.0 ** -8 * (want.abs() + bound)
+        assert ((out[i].double() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize('rows,hidden', ((1, 16), (3, 528), (129, 1040)))
 @pytest.mark.parametrize('dtype', (torch.bfloat16, torch.float32), ids=('bf16', 'fp32'))
 def test_nvfp4_writes_its_output_only(cuda_device, rows, hidden, dtype):
